@@ -8,9 +8,15 @@ Public API (same names and behaviour as the reference package ``dot``,
     P = bidirectional_softmax(sim_matrix, tau=1.0)
 
 plus the nn.Module wrappers ``Sinkhorn``, ``SinkhornFromScores`` and
-``BidirectionalSoftmax``, and one extension with no counterpart in the
+``BidirectionalSoftmax``, and extensions with no counterpart in the
 reference: ``sinkhorn_points(x, y, reg, n_iters)``, Sinkhorn on two point
-clouds with the squared-distance cost built inside the solver.  Low-level
+clouds with the squared-distance cost built inside the solver, and two
+operators for the features a matching is computed from,
+
+    y = group_norm_act(x, num_groups, weight, bias, activation="silu")
+    q, k = rotary(q, positions, freqs, k=k)
+
+(modules ``GroupNormAct`` and ``Rotary``).  Low-level
 operators mirroring the reference's ``dot._ops`` live in
 :mod:`dot_b200.ops`; the C-ABI they call is
 ``include/dot_b200.h``.  Importing the package loads the native library and
@@ -27,7 +33,9 @@ from .bidirectional_softmax import (  # noqa: E402
     bidirectional_softmax,
     bidirectional_softmax_with_lengths,
 )
+from .norm import GroupNormAct, group_norm_act  # noqa: E402
 from .points import sinkhorn_points  # noqa: E402
+from .rotary import Rotary, rotary, rotary_freqs  # noqa: E402
 from .sinkhorn import (  # noqa: E402
     Sinkhorn,
     SinkhornFromScores,
@@ -48,4 +56,9 @@ __all__ = [
     "bidirectional_softmax_with_lengths",
     "BidirectionalSoftmax",
     "sinkhorn_points",
+    "group_norm_act",
+    "GroupNormAct",
+    "rotary",
+    "rotary_freqs",
+    "Rotary",
 ]

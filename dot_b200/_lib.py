@@ -16,9 +16,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libdot_b200.so")
 ABI_VERSION = 1
 
-DOT_F32, DOT_BF16, DOT_F16 = 0, 1, 2
+DOT_F32, DOT_BF16, DOT_F16, DOT_I32, DOT_I64 = 0, 1, 2, 3, 4
+ACTIVATIONS = ("none", "silu", "gelu", "relu")   # enum dot_activation
 KCLASSES = ("sk_fwd_iter", "sk_fwd_epi", "sk_bwd_iter", "sk_bwd_epi", "sk_resident", "bs_fwd", "bs_bwd",
-            "sk_exchange")
+            "sk_exchange", "norm_fwd", "norm_bwd", "rotary")
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -65,8 +66,17 @@ _SIGS = {
     "dot_bidir_fwd": (_i, [_vp, _i, _vp, _i64, _i64, _i64, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "dot_bidir_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "dot_bidir_bwd": (_i, [_vp, _i, _vp, _i64, _i64, _i64, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "dot_group_norm_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "dot_group_norm_fwd": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _i, _vp, _i64, _i64, _i64, _i64, _f, _i, _vp, _vp,
+                                _vp, _sz, _vp]),
+    "dot_group_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "dot_group_norm_bwd": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _vp, _i64, _i64, _i64, _i64, _i,
+                                _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dot_rotary": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i, _vp, _i, _vp, _vp, _i64, _i64, _i64, _i64, _i, _i, _i,
+                        _vp, _vp, _vp]),
     "dot_prof_begin": (_i, [_i]),
     "dot_prof_end": (_i, [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_double)]),
+    "dot_prof_end_n": (_i, [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_double), _i]),
 }
 
 _lib = None
@@ -129,5 +139,5 @@ def prof_end() -> dict:
     n = len(KCLASSES)
     launches = (ctypes.c_int64 * n)()
     ms = (ctypes.c_double * n)()
-    check(load().dot_prof_end(launches, ms), "dot_prof_end")
+    check(load().dot_prof_end_n(launches, ms, n), "dot_prof_end_n")
     return {k: {"launches": int(launches[i]), "ms": float(ms[i])} for i, k in enumerate(KCLASSES)}

@@ -46,14 +46,14 @@ namespace {
 struct Prof {
     std::mutex mu;
     bool timing = false;
-    int64_t launches[DOT_K_NCLASS] = {};
+    int64_t launches[DOT_K_NCLASS_ALL] = {};
     struct Pair {
         int k;
         cudaEvent_t a, b;
     };
     std::vector<Pair> pairs;
     std::vector<cudaEvent_t> pool;
-    cudaEvent_t pending[DOT_K_NCLASS] = {};
+    cudaEvent_t pending[DOT_K_NCLASS_ALL] = {};
 };
 Prof& prof() {
     static Prof p;
@@ -424,7 +424,7 @@ int dot_prof_begin(int time_events) {
     clear_error();
     Prof& p = prof();
     std::lock_guard<std::mutex> g(p.mu);
-    for (int k = 0; k < DOT_K_NCLASS; ++k) p.launches[k] = 0;
+    for (int k = 0; k < DOT_K_NCLASS_ALL; ++k) p.launches[k] = 0;
     for (auto& pr : p.pairs) {
         p.pool.push_back(pr.a);
         p.pool.push_back(pr.b);
@@ -434,11 +434,14 @@ int dot_prof_begin(int time_events) {
     return DOT_OK;
 }
 
-int dot_prof_end(int64_t* launches, double* ms) {
+int dot_prof_end(int64_t* launches, double* ms) { return dot_prof_end_n(launches, ms, DOT_K_NCLASS); }
+
+int dot_prof_end_n(int64_t* launches, double* ms, int n) {
     clear_error();
+    if (n < 0 || n > DOT_K_NCLASS_ALL) return fail(DOT_ERR_INVALID, "unknown number of kernel classes");
     Prof& p = prof();
     std::lock_guard<std::mutex> g(p.mu);
-    double acc[DOT_K_NCLASS] = {};
+    double acc[DOT_K_NCLASS_ALL] = {};
     for (auto& pr : p.pairs) {
         if (cudaEventSynchronize(pr.b) != cudaSuccess) return fail(DOT_ERR_CUDA, "event synchronize failed");
         float t = 0.0f;
@@ -449,7 +452,7 @@ int dot_prof_end(int64_t* launches, double* ms) {
     }
     p.pairs.clear();
     p.timing = false;
-    for (int k = 0; k < DOT_K_NCLASS; ++k) {
+    for (int k = 0; k < n; ++k) {
         if (launches) launches[k] = p.launches[k];
         if (ms) ms[k] = acc[k];
     }

@@ -19,7 +19,9 @@ All ops run on CUDA tensors only and enqueue on the current stream.
 
 from __future__ import annotations
 
+import functools
 import math
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -217,6 +219,133 @@ def sinkhorn_points_forward_raw(x: torch.Tensor, y: torch.Tensor, cost_scale: fl
                                      nbytes, _lib.stream_of(x))
     _lib.check(rc, "dot_sinkhorn_points_fwd")
     return plan, cost, u, v, status
+
+
+# ---- feature operators ----------------------------------------------------------
+
+_FEATURE_DTYPES = {torch.float32: _lib.DOT_F32, torch.bfloat16: _lib.DOT_BF16, torch.float16: _lib.DOT_F16}
+_POSITION_DTYPES = {torch.int32: _lib.DOT_I32, torch.int64: _lib.DOT_I64, torch.float32: _lib.DOT_F32}
+
+
+def _on(t: torch.Tensor):
+    """Makes ``t``'s device current for a launch, where it is not."""
+    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _rows(x: torch.Tensor):
+    """``x`` [N, *S, C] as ``(x, N, S, C, batch stride, position stride)``: a view whose channels are
+    consecutive and whose positions lie at one stride is read in place, anything else is copied."""
+    N, C = x.size(0), x.size(-1)
+    if x.numel() == 0:
+        return x, N, math.prod(x.shape[1:-1]), C, 0, 0
+    S = x.numel() // (N * C)
+    if x.is_contiguous():
+        return x, N, S, C, S * C, C
+    one, step = x.stride(-1), 0
+    for size, stride in zip(reversed(x.shape[1:-1]), reversed(x.stride()[1:-1])):
+        if size == 1:
+            continue
+        if step == 0:
+            step, span = stride, stride * size
+        elif stride != span:
+            step = -1
+            break
+        else:
+            span = stride * size
+    if step < 0 or (C > 1 and one != 1):
+        return x.contiguous(), N, S, C, S * C, C
+    return x, N, S, C, x.stride(0), step
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace_bytes(N: int, S: int, C: int, G: int, backward: bool) -> int:
+    lib = _lib.load()
+    return (lib.dot_group_norm_bwd_workspace_bytes if backward else lib.dot_group_norm_fwd_workspace_bytes)(N, S, C, G)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def group_norm_forward_raw(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor],
+                           bias: Optional[torch.Tensor], eps: float, activation: int,
+                           lengths: Optional[torch.Tensor] = None):
+    """One call of ``dot_group_norm_fwd`` on x [N, *S, C]; returns ``(y, stats [N,G,2])``."""
+    x, N, S, C, xb, xp = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((N, num_groups, 2), dtype=torch.float32, device=x.device)
+    nbytes = _norm_workspace_bytes(N, S, C, num_groups, False)
+    ws = _lib.workspace(nbytes, x.device)
+    p = weight if weight is not None else bias
+    with _on(x):
+        rc = _lib.load().dot_group_norm_fwd(
+            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, _ptr(weight), _ptr(bias),
+            _lib.DOT_F32 if p is None else _FEATURE_DTYPES[p.dtype], _ptr(lengths), N, S, C, num_groups, eps,
+            activation, y.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes, _lib.stream_of(x))
+    if rc:
+        _lib.check(rc, "dot_group_norm_fwd")
+    return y, stats
+
+
+def group_norm_backward_raw(x: torch.Tensor, dy: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor],
+                            bias: Optional[torch.Tensor], activation: int, stats: torch.Tensor,
+                            lengths: Optional[torch.Tensor] = None, want_dx: bool = True,
+                            want_dweight: bool = True, want_dbias: bool = True):
+    """One call of ``dot_group_norm_bwd``; returns ``(dx, dweight, dbias)``, None where not wanted."""
+    x, N, S, C, xb, xp = _rows(x)
+    dy, _, _, _, gb, gp = _rows(dy)
+    p = weight if weight is not None else bias
+    pdt = torch.float32 if p is None else p.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty((C,), dtype=pdt, device=x.device) if want_dweight else None
+    db = torch.empty((C,), dtype=pdt, device=x.device) if want_dbias else None
+    nbytes = _norm_workspace_bytes(N, S, C, num_groups, True)
+    ws = _lib.workspace(nbytes, x.device)
+    with _on(x):
+        rc = _lib.load().dot_group_norm_bwd(
+            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, dy.data_ptr(), gb, gp, _ptr(weight), _ptr(bias),
+            _FEATURE_DTYPES[pdt], _ptr(lengths), N, S, C, num_groups, activation, stats.data_ptr(), _ptr(dx),
+            _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_of(x))
+    if rc:
+        _lib.check(rc, "dot_group_norm_bwd")
+    return dx, dw, db
+
+
+def _heads(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with consecutive elements within a head."""
+    return x if x.stride(-1) == 1 or x.size(-1) == 1 else x.contiguous()
+
+
+def _i64x3(a: int, b: int, c: int):
+    return (_lib.ctypes.c_int64 * 3)(a, b, c)
+
+
+def rotary_raw(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
+               interleaved: bool, inverse: bool = False):
+    """One call of ``dot_rotary`` on q [B,L,Hq,D] and/or k [B,L,Hk,D] with positions [B or 1, L, A] and
+    freqs [P,A]; returns ``(q', k')``, None where the input is None."""
+    ref = q if q is not None else k
+    B, L, _, D = ref.shape
+    outs, args = [], []
+    for t in (q, k):
+        if t is None:
+            outs.append(None)
+            args.append((None, None, 0))
+            continue
+        t = _heads(t)
+        outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
+        args.append((t, _i64x3(t.stride(0), t.stride(1), t.stride(2)), t.size(2)))
+    (q, qs, hq), (k, ks, hk) = args
+    P, A = freqs.shape
+    ps = _i64x3(positions.stride(0) if positions.size(0) == B else 0, positions.stride(1), positions.stride(2))
+    with _on(ref):
+        rc = _lib.load().dot_rotary(
+            _ptr(q), qs, hq, _ptr(k), ks, hk, _FEATURE_DTYPES[ref.dtype], positions.data_ptr(),
+            _POSITION_DTYPES[positions.dtype], ps, freqs.data_ptr(), B, L, D, P, A, 1 if interleaved else 0,
+            1 if inverse else 0, _ptr(outs[0]), _ptr(outs[1]), _lib.stream_of(ref))
+    if rc:
+        _lib.check(rc, "dot_rotary")
+    return outs[0], outs[1]
 
 
 # ---- reference-named ops ------------------------------------------------------

@@ -44,7 +44,10 @@ enum dot_status {
     DOT_ERR_UNSUPPORTED = -4  /* valid request this build does not implement    */
 };
 
-enum dot_dtype { DOT_F32 = 0, DOT_BF16 = 1, DOT_F16 = 2 };
+enum dot_dtype { DOT_F32 = 0, DOT_BF16 = 1, DOT_F16 = 2, DOT_I32 = 3, DOT_I64 = 4 };
+
+/* Activations of dot_group_norm_fwd / _bwd (gelu is the exact, erf form). */
+enum dot_activation { DOT_ACT_NONE = 0, DOT_ACT_SILU = 1, DOT_ACT_GELU = 2, DOT_ACT_RELU = 3 };
 
 /* Text of the calling thread's last error ("" if none). */
 DOT_API const char* dot_last_error(void);
@@ -361,6 +364,71 @@ DOT_API int dot_bidir_bwd(const void* sim, int sim_dtype, const int32_t* lengths
                   void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Feature operators (no counterpart in the reference)                       */
+/* ------------------------------------------------------------------------ */
+
+/* Bytes of workspace dot_group_norm_fwd / _bwd need for this problem. */
+DOT_API size_t dot_group_norm_fwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G);
+DOT_API size_t dot_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G);
+
+/*
+ * Group normalisation with an activation on channels-last features: for each
+ * sample n and group g of C/G consecutive channels, mean and (biased) variance
+ * over the group's channels at the sample's positions i < lengths[n], then
+ *     z = (x - mean) / sqrt(var + eps) * weight_c + bias_c,   y = act(z),
+ * and y = 0 at positions i >= lengths[n], whose x is never read.
+ * x: S positions of C consecutive elements per sample, x_batch_stride and
+ * x_pos_stride elements from one sample / position to the next (a slice of
+ * wider rows is read in place); y is dense [N,S,C] of x's dtype (DOT_F32,
+ * DOT_BF16 or DOT_F16; computed in fp32, rounded once).  weight, bias [C] of
+ * param_dtype (each may be NULL: 1 and 0).  lengths: device int32 [N], clamped
+ * to [0, S] (NULL: all S).  stats [N,G,2] fp32 receives (mean,
+ * 1/sqrt(var + eps)) for the backward ((0, 1/sqrt(eps)) where nothing is valid).
+ */
+DOT_API int dot_group_norm_fwd(const void* x, int dtype, int64_t x_batch_stride, int64_t x_pos_stride,
+                               const void* weight, const void* bias, int param_dtype,
+                               const int32_t* lengths, int64_t N, int64_t S, int64_t C, int64_t G,
+                               float eps, int activation, void* y, float* stats, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
+ * Backward of dot_group_norm_fwd for the upstream dy (strides as x's, same
+ * dtype), with xh = (x - mean) rstd and dz = dy act'(xh weight + bias):
+ *     dbias_c = sum_{n,i} dz,   dweight_c = sum_{n,i} dz xh,
+ *     dx = rstd (weight dz - mean_g(weight dz) - xh mean_g(weight dz xh)),
+ * sums and means over valid positions (mean_g also over the group's
+ * channels); dx [N,S,C] dense, 0 at positions i >= lengths[n].  dx, dweight
+ * and dbias may each be NULL; the latter are written as param_dtype.  Sums are
+ * taken in a fixed order (results are bitwise reproducible).
+ */
+DOT_API int dot_group_norm_bwd(const void* x, int dtype, int64_t x_batch_stride, int64_t x_pos_stride,
+                               const void* dy, int64_t dy_batch_stride, int64_t dy_pos_stride,
+                               const void* weight, const void* bias, int param_dtype,
+                               const int32_t* lengths, int64_t N, int64_t S, int64_t C, int64_t G,
+                               int activation, const float* stats, void* dx, void* dweight, void* dbias,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions with several axes: token (b, l) has the angles
+ *     angle_p = sum_{a < A} positions[b,l,a] * freqs[p,a],   p < P,
+ * and pair p of each of its heads, (x_p, x_{P+p}) or with interleaved != 0
+ * (x_2p, x_{2p+1}), becomes (x cos - y sin, y cos + x sin); elements from 2P
+ * on are copied.  inverse != 0 turns by -angle (the backward).
+ * q [B,L,Hq,D] and k [B,L,Hk,D] (k may be NULL with Hk = 0) share the angles;
+ * each is given with its strides in elements {b, l, h} (host arrays) and
+ * consecutive elements within a head; q_out, k_out are dense.  dtype DOT_F32,
+ * DOT_BF16 or DOT_F16.  positions: DOT_I32, DOT_I64 or DOT_F32 with strides
+ * {b, l, a} (0 repeats it along b); freqs: fp32 [P,A], 1 <= A <= 4.
+ * The angle is formed in fp64 and reduced to one turn before its sine and
+ * cosine are taken in fp32, so long positions lose nothing.
+ */
+DOT_API int dot_rotary(const void* q, const int64_t* q_strides, int64_t Hq, const void* k,
+                       const int64_t* k_strides, int64_t Hk, int dtype, const void* positions,
+                       int pos_dtype, const int64_t* pos_strides, const float* freqs, int64_t B,
+                       int64_t L, int64_t D, int64_t P, int A, int interleaved, int inverse, void* q_out,
+                       void* k_out, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Instrumentation (no counterpart in the reference)                         */
 /* ------------------------------------------------------------------------ */
 
@@ -375,7 +443,11 @@ enum dot_kclass {
     DOT_K_BS_BWD = 6,        /* bidirectional softmax backward               */
     DOT_K_SK_EXCHANGE = 7,   /* row-shard column exchange: pair merges and   */
                              /* the all-gather between the shards            */
-    DOT_K_NCLASS = 8
+    DOT_K_NCLASS = 8,        /* the classes dot_prof_end reports            */
+    DOT_K_NORM_FWD = 8,      /* group norm with an activation               */
+    DOT_K_NORM_BWD = 9,
+    DOT_K_ROTARY = 10,       /* rotary positions                             */
+    DOT_K_NCLASS_ALL = 11    /* all classes (dot_prof_end_n)                 */
 };
 
 /* Start counting launches per class; with time_events != 0 also bracket each
@@ -386,6 +458,9 @@ DOT_API int dot_prof_begin(int time_events);
  * milliseconds (arrays of DOT_K_NCLASS entries; either may be NULL).
  * Synchronises the recorded events. */
 DOT_API int dot_prof_end(int64_t* launches, double* ms);
+
+/* dot_prof_end for arrays of n entries: the first n classes (n <= DOT_K_NCLASS_ALL). */
+DOT_API int dot_prof_end_n(int64_t* launches, double* ms, int n);
 
 #ifdef __cplusplus
 }
