@@ -68,7 +68,7 @@ int dot_group_norm_fwd(const void* x, int dtype, int64_t x_batch_stride, int64_t
     a.param_dtype = param_dtype;
     a.act = activation;
     a.eps = eps;
-    return gn_fwd(a, workspace, static_cast<cudaStream_t>(stream));
+    return gn_run(a, workspace, false, static_cast<cudaStream_t>(stream));
 }
 
 int dot_group_norm_bwd(const void* x, int dtype, int64_t x_batch_stride, int64_t x_pos_stride, const void* dy,
@@ -112,7 +112,7 @@ int dot_group_norm_bwd(const void* x, int dtype, int64_t x_batch_stride, int64_t
     a.dtype = dtype;
     a.param_dtype = param_dtype;
     a.act = activation;
-    return gn_bwd(a, workspace, st);
+    return gn_run(a, workspace, true, st);
 }
 
 int dot_rotary(const void* q, const int64_t* q_strides, int64_t Hq, const void* k, const int64_t* k_strides,

@@ -23,6 +23,10 @@ __device__ __forceinline__ uint32_t cl_id() {
 __device__ __forceinline__ void cl_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of cl_sync: what a thread wrote before arriving is visible to
+// the cluster's threads after they waited.
+__device__ __forceinline__ void cl_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cl_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // 4 bytes into another CTA's shared memory; they complete a transaction on
 // that CTA's mbarrier.
 __device__ __forceinline__ void st_async_f32(uint32_t remote_addr, uint32_t remote_bar, float v) {
@@ -33,6 +37,11 @@ __device__ __forceinline__ void st_async_f32(uint32_t remote_addr, uint32_t remo
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t ld_cluster_u16(uint32_t addr) {

@@ -54,6 +54,20 @@ __device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
     return p;
 }
 
+// Makes a register's bits opaque, so that what was computed from them is not
+// kept alive across this point but computed again (a 16-bit vector costs half
+// the registers of its float32 values).
+template <typename T, int N>
+__device__ __forceinline__ void reload(Pack<T, N>& p) {
+    if constexpr (sizeof(p) >= 4) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+        for (int i = 0; i < int(sizeof(p) / 4); ++i) asm volatile("" : "+r"(w[i]));
+    } else {
+        asm volatile("" : "+h"(*reinterpret_cast<uint16_t*>(&p)));
+    }
+}
+
 // A per-channel parameter of type `dtype` (enum dot_dtype).
 __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
     if (dtype == 0) return static_cast<const float*>(p)[i];

@@ -28,8 +28,11 @@ struct GroupNormArgs {
 
 size_t gn_fwd_ws(int64_t N, int64_t S, int64_t C, int64_t G);
 size_t gn_bwd_ws(int64_t N, int64_t S, int64_t C, int64_t G);
-int gn_fwd(const GroupNormArgs& a, void* ws, cudaStream_t st);
-int gn_bwd(const GroupNormArgs& a, void* ws, cudaStream_t st);
+int gn_run(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st);
+// one unit per element type
+int gn_f32(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st);
+int gn_bf16(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st);
+int gn_f16(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st);
 
 constexpr int kMaxAxes = 4;
 
