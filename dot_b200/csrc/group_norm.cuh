@@ -33,26 +33,29 @@
 namespace dotb {
 namespace {
 
-constexpr int kGnThreads = 256;
+constexpr int kSMs = 148;
+// One block of 512 threads per SM: up to 128 registers a thread, so that enough
+// loads are in flight (8 of 16 bytes a thread, 64 KB per SM).
+constexpr int kGnThreads = 512;
 constexpr int kGnWarps = kGnThreads / 32;
-
-// Resident path: threads of a block, and the registers of a thread that hold
-// x (and as many dy): vectors of 16 bytes or fewer.
-constexpr int kResThreads = 512;
 constexpr int kMaxCluster = 8;
-constexpr int res_vecs(int bytes) { return bytes >= 16 ? 8 : bytes >= 8 ? 16 : 32; }
+
+// Resident path: vectors that a thread keeps of x (forward), or of x and of dy.
+constexpr int res_vecs(int bytes, bool backward) {
+    const int n = bytes >= 16 ? 8 : bytes >= 8 ? 16 : 32;
+    return backward || n == 32 ? n : 2 * n;
+}
 
 struct GnPlan {
     GroupNormArgs a;
     int n0;              // sweeps: first sample of this launch
     int chunks;          // blocks that share a sample's positions
     int rows;            // positions per chunk
-    int parts;           // partial sums per sample in the workspace
     int slab_groups;     // resident: groups of a block's channel slab
     int slabs;           // resident: slabs per sample
-    float2* moments;     // sweeps, fwd: [N][parts][G] (mean, M) of a cluster
-    float2* gsums;       // sweeps, bwd: [N][parts][G] (sum w dz, sum w dz xh)
-    float2* csums;       // bwd: [N][parts][C] (sum dz, sum dz xh)
+    float2* moments;     // sweeps, fwd: [N][chunks][G] (mean, M) of a chunk
+    float2* gsums;       // sweeps, bwd: [N][chunks][G] (sum w dz, sum w dz xh)
+    float2* csums;       // bwd: [N][chunks][C] (sum dz, sum dz xh)
 };
 
 // Merging partial moments (mean_i, M_i) of n_i values each about one of the
@@ -60,24 +63,55 @@ struct GnPlan {
 //   mean = about + sum n_i d_i / n,   M = sum (M_i + n_i d_i^2) - (sum n_i d_i)^2 / n.
 // What cancels in M is at most n / n_i of it, from that mean's own distance.
 struct Merge {
-    float n = 0.0f, nd = 0.0f, m2 = 0.0f;
+    float nd = 0.0f, m2 = 0.0f;
     __device__ __forceinline__ void add(float about, float ni, float mean, float m) {
         const float d = mean - about, w = ni * d;
         if (ni > 0.0f) {   // the moments of nothing are not looked at
-            n += ni;
             nd += w;
             m2 += m + w * d;
         }
     }
-    __device__ __forceinline__ void warp() {
-        n = warp_sum<32>(n);
-        nd = warp_sum<32>(nd);
-        m2 = warp_sum<32>(m2);
+    // over 2^log lanes of a warp
+    __device__ __forceinline__ void lanes(int log) {
+        for (int off = (1 << log) >> 1; off > 0; off >>= 1) {
+            nd += __shfl_xor_sync(0xffffffffu, nd, off);
+            m2 += __shfl_xor_sync(0xffffffffu, m2, off);
+        }
     }
-    // (mean, M)
-    __device__ __forceinline__ float2 pair(float about) const {
+    // (mean, M) of n values
+    __device__ __forceinline__ float2 pair(float about, float n) const {
         const float d = n > 0.0f ? nd / n : 0.0f;
         return n > 0.0f ? make_float2(about + d, m2 - nd * d) : make_float2(0.0f, 0.0f);
+    }
+};
+
+__device__ __forceinline__ float2 lanes_sum(float2 s, int log) {
+    for (int off = (1 << log) >> 1; off > 0; off >>= 1) {
+        s.x += __shfl_xor_sync(0xffffffffu, s.x, off);
+        s.y += __shfl_xor_sync(0xffffffffu, s.y, off);
+    }
+    return s;
+}
+
+// How many lanes a block gives each of `count` groups: the largest power of two
+// (as its logarithm) that leaves none waiting, at most a warp.
+__device__ __forceinline__ int lanes_log(int count, int threads) {
+    int log = 5;
+    while (log > 0 && (count << log) > threads) --log;
+    return log;
+}
+
+// The group of each of a thread's channels c, c + 1, ...: one division.
+struct GroupOf {
+    int g, left, Cg;
+    __device__ GroupOf(int c, int Cg_) : g(c / Cg_), left(Cg_ - (c - g * Cg_)), Cg(Cg_) {}
+    __device__ __forceinline__ int next() {   // the current channel's group, then on to the next channel
+        const int now = g;
+        if (--left == 0) {
+            left = Cg;
+            ++g;
+        }
+        return now;
     }
 };
 
@@ -98,14 +132,113 @@ __device__ __forceinline__ int valid_len(const GroupNormArgs& a, int n) {
     return int(min(max(int64_t(__ldg(a.lengths + n)), int64_t(0)), a.S));
 }
 
-// dx of one element from its group's statistics and sums (S1/m, S2/m).  w dz is
-// rounded as in its sum: the gradient of a group of one value is 0.
-template <int ACT>
-__device__ __forceinline__ float dx_of(float x, float dy, float mean, float rstd, float w, float b, float2 s, int act) {
-    const float xh = (x - mean) * rstd;
-    const float dz = dy * act_slope<ACT>(xh * w + b, act);
-    return rstd * (__fsub_rn(__fmul_rn(w, dz), s.x) - xh * s.y);
-}
+// A thread's channels: per-channel parameters in pairs, a group's values once
+// where the vector lies in one group.
+template <int VEC, bool ONEG>
+struct PerGroup {
+    static constexpr int NP = pairs_of(VEC);
+    float2 v[ONEG ? 1 : NP];
+    __device__ __forceinline__ float2 operator[](int j) const { return v[ONEG ? 0 : j]; }
+    // f(g): the value of group g; c: the first channel
+    template <typename F>
+    __device__ __forceinline__ void fill(int c, int Cg, F f) {
+        GroupOf of(c, Cg);
+        if constexpr (ONEG) {
+            v[0] = splat2(f(of.g));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                v[j].x = f(of.next());
+                v[j].y = VEC == 1 ? 0.0f : f(of.next());
+            }
+        }
+    }
+};
+
+// y of a vector.  16-bit values take the mean with the shift (one fma); float32
+// subtracts it first, since the rounding of a large mean * scale would show.
+template <typename T, int VEC, int ACT, bool ONEG>
+struct Forward {
+    static constexpr int NP = pairs_of(VEC);
+    static constexpr bool FOLD = sizeof(T) == 2;
+    PerGroup<VEC, ONEG || FOLD> mean;   // unused where folded
+    float2 scale[NP], shift[NP];
+    // st: (mean, rstd) by group; c: the first channel, c_st: counted from st's first group
+    __device__ __forceinline__ void load(const GroupNormArgs& a, int c, int c_st, int Cg, const float2* st) {
+        load_params<VEC>(a.weight, a.param_dtype, c, 1.0f, scale);
+        load_params<VEC>(a.bias, a.param_dtype, c, 0.0f, shift);
+        PerGroup<VEC, ONEG> m, r;
+        m.fill(c_st, Cg, [&](int g) { return st[g].x; });
+        r.fill(c_st, Cg, [&](int g) { return st[g].y; });
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            scale[j] = mul2(scale[j], r[j]);
+            if constexpr (FOLD)
+                shift[j] = fma2(make_float2(-m[j].x, -m[j].y), scale[j], shift[j]);
+            else
+                mean.v[ONEG ? 0 : j] = m[j];
+        }
+    }
+    __device__ __forceinline__ Pack<T, VEC> operator()(const Pack<T, VEC>& raw, int act) const {
+        float2 f[NP];
+        unpack(raw, f);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+            f[j] = act_fwd<ACT>(fma2(FOLD ? f[j] : sub2(f[j], mean[j]), scale[j], shift[j]), act);
+        return pack<T, VEC>(f);
+    }
+};
+
+// The backward's chain for a vector: xh, dz; the sums of dz and dz xh; dx.
+template <typename T, int VEC, int ACT, bool ONEG>
+struct Backward {
+    static constexpr int NP = pairs_of(VEC);
+    PerGroup<VEC, ONEG> mean, rstd;
+    float2 w[NP], b[NP];
+    // st: a pair or more by group, mean and rstd first; c_st: c counted from st's first group
+    template <typename S>
+    __device__ __forceinline__ void load(const GroupNormArgs& a, int c, int c_st, int Cg, const S* st) {
+        load_params<VEC>(a.weight, a.param_dtype, c, 1.0f, w);
+        load_params<VEC>(a.bias, a.param_dtype, c, 0.0f, b);
+        mean.fill(c_st, Cg, [&](int g) { return st[g].x; });
+        rstd.fill(c_st, Cg, [&](int g) { return st[g].y; });
+    }
+    __device__ __forceinline__ void chain(float2 x, float2 dy, int j, int act, float2& xh, float2& dz) const {
+        xh = mul2(sub2(x, mean[j]), rstd[j]);
+        dz = mul2(dy, act_slope<ACT>(fma2(xh, w[j], b[j]), act));
+    }
+    __device__ __forceinline__ void sums(const Pack<T, VEC>& rx, const Pack<T, VEC>& rg, int act, float2 (&sa)[NP],
+                                         float2 (&sb)[NP]) const {
+        float2 x[NP], g[NP];
+        unpack(rx, x);
+        unpack(rg, g);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            float2 xh, dz;
+            chain(x[j], g[j], j, act, xh, dz);
+            sa[j] = add2(sa[j], dz);
+            sb[j] = fma2(dz, xh, sb[j]);
+        }
+    }
+    // s1, s2: the group's S1/m and S2/m
+    __device__ __forceinline__ Pack<T, VEC> dx(const Pack<T, VEC>& rx, const Pack<T, VEC>& rg, int act,
+                                               const PerGroup<VEC, ONEG>& s1, const PerGroup<VEC, ONEG>& s2) const {
+        float2 x[NP], g[NP];
+        unpack(rx, x);
+        unpack(rg, g);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            float2 xh, dz;
+            chain(x[j], g[j], j, act, xh, dz);
+            // w dz rounded as in its sum (a scalar product is not contracted): the
+            // gradient of a group of one value is 0
+            const float2 wdz = make_float2(__fmul_rn(w[j].x, dz.x), __fmul_rn(w[j].y, dz.y));
+            const float2 t = sub2(wdz, s1[j]), n = mul2(xh, splat2(-1.0f));
+            x[j] = mul2(rstd[j], fma2(n, s2[j], t));
+        }
+        return pack<T, VEC>(x);
+    }
+};
 
 // ---- backward: the parameters' gradients from the blocks' channel sums ---------
 __global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
@@ -113,9 +246,10 @@ __global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
     __shared__ float2 part[kGnWarps][32];
     const int C = int(a.C), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
-    const int64_t rows = a.N * pl.parts;
+    const int64_t rows = a.N * pl.chunks;
     float2 s = make_float2(0.0f, 0.0f);
     if (c < C)
+#pragma unroll 8
         for (int64_t r = warp; r < rows; r += kGnWarps) {
             const float2 v = pl.csums[r * C + c];
             s.x += v.x;
@@ -140,10 +274,6 @@ __global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
 // merges its sample's partials at its start and writes the result, walking its
 // rows backwards: it begins with those that the first sweep read last.
 
-// Clusters of kSweepCluster blocks join their partials through distributed
-// shared memory first, so a sample's chunks leave an eighth as many.
-constexpr int kSweepCluster = 8;
-
 // Valid positions of chunk k of `rows`.
 __device__ __forceinline__ int rows_of(int len, int k, int rows) { return min(max(len - k * rows, 0), rows); }
 
@@ -161,50 +291,77 @@ struct Place {
     }
 };
 
-// A running (count of positions, mean, M) per channel, or one for a vector
-// that lies in one group.
-template <int VEC, bool ONEG>
-struct Running {
-    static constexpr int NG = ONEG ? 1 : VEC;
-    float n = 0.0f, mean[NG], m2[NG];
-    __device__ Running() {
+// Mean (about the pivot) and M of the first `k` of U vectors of a thread, per
+// channel, or one for all channels of a vector that lies in one group: two
+// passes over the registers.  The sum of a batch of 16-bit values is taken as
+// it is (their few bits leave its rounding far below the pivot's), float32
+// subtracts the pivot first.
+template <typename T, int VEC, bool ONEG>
+struct Batch {
+    static constexpr int NP = pairs_of(VEC), NG = ONEG ? 1 : VEC;
+    float mean[NG], m2[NG];
+    template <int U, bool FULL>
+    __device__ __forceinline__ void take(Pack<T, VEC> (&raw)[U], const PerGroup<VEC, ONEG>& pivot, int k) {
+        constexpr bool RAW = sizeof(T) == 2;
+        const float inv = (FULL ? 1.0f / float(U) : 1.0f / float(k > 0 ? k : 1)) * (ONEG ? 1.0f / float(VEC) : 1.0f);
+        float2 s[NP], q[NP], about[NP];
 #pragma unroll
-        for (int j = 0; j < NG; ++j) mean[j] = m2[j] = 0.0f;
-    }
-    // Merges the first k of U positions, by two passes over registers.
-    template <typename T, int U, bool FULL>
-    __device__ __forceinline__ void add(const Pack<T, VEC> (&raw)[U], const float (&pivot)[NG], int k) {
-        constexpr int J = ONEG ? VEC : 1;   // values of a position in a pair
-        const float fk = FULL ? float(U) : float(k), tot = n + fk, f = fk / tot, w = n * f;
-        const float inv = (FULL ? 1.0f / float(U) : 1.0f / fk) * (1.0f / float(J));
+        for (int j = 0; j < NP; ++j) s[j] = q[j] = splat2(0.0f);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float s = 0.0f, q = 0.0f;
+        for (int u = 0; u < U; ++u)
+            if (FULL || u < k) {
+                float2 f[NP];
+                unpack(raw[u], f);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (FULL || u < k)
+                for (int j = 0; j < NP; ++j) s[j] = add2(s[j], RAW ? f[j] : sub2(f[j], pivot[j]));
+            }
+        if constexpr (ONEG) {
+            const float2 t = tree_sum2(s);
+            const float all = VEC == 1 ? t.x : t.x + t.y;
+            const float p = pivot[0].x;
+            mean[0] = RAW ? fmaf(all, inv, -p) : all * inv;
 #pragma unroll
-                    for (int j = 0; j < J; ++j) s += to_f32(raw[u].v[g + j]) - pivot[g];
-            s *= inv;
+            for (int j = 0; j < NP; ++j) about[j] = splat2(p + mean[0]);
+        } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (FULL || u < k)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        const float d = (to_f32(raw[u].v[g + j]) - pivot[g]) - s;
-                        q += d * d;
-                    }
-            const float d = s - mean[g];
-            mean[g] += d * f;
-            m2[g] += q + d * d * (w * float(J));
+            for (int j = 0; j < NP; ++j) {
+                const float2 p = pivot[j];
+                const float2 m = RAW ? fma2(s[j], splat2(inv), make_float2(-p.x, -p.y)) : mul2(s[j], splat2(inv));
+                about[j] = add2(p, m);
+                mean[2 * j] = m.x;
+                if constexpr (VEC > 1) mean[2 * j + 1] = m.y;
+            }
         }
-        n = tot;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (U > 4) reload(raw[u]);
+            if (FULL || u < k) {
+                float2 f[NP];
+                unpack(raw[u], f);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    const float2 d = sub2(f[j], about[j]);
+                    q[j] = fma2(d, d, q[j]);
+                }
+            }
+            if (U > 4) reload(raw[u]);
+        }
+        if constexpr (ONEG) {
+            const float2 t = tree_sum2(q);
+            m2[0] = VEC == 1 ? t.x : t.x + t.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                m2[2 * j] = q[j].x;
+                if constexpr (VEC > 1) m2[2 * j + 1] = q[j].y;
+            }
+        }
     }
 };
 
 // Forward, sweep 1: moments of every group over a chunk.
 template <typename T, int VEC, bool ONEG>
-__global__ void __launch_bounds__(kGnThreads) gn_moments_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     constexpr int W = ONEG ? 1 : VEC, U = 8;
@@ -215,25 +372,37 @@ __global__ void __launch_bounds__(kGnThreads) gn_moments_kernel(GnPlan pl) {
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
         const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
         if (pc.on) {
-            Running<VEC, ONEG> run;
+            PerGroup<VEC, ONEG> pivot;
+            pivot.fill(c0 + pc.v * VEC, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
             const T* xc = x + c0 + pc.v * VEC;
-            float pivot[W];
-#pragma unroll
-            for (int j = 0; j < W; ++j) pivot[j] = group_pivot(x, len, (c0 + pc.v * VEC + j) / Cg * Cg);
             const int64_t step = int64_t(pc.rp) * a.xp;
+            float n_run = 0.0f, mean[W], m2[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) mean[j] = m2[j] = 0.0f;
+            Batch<T, VEC, ONEG> bt;
+            auto join = [&](float k) {
+                const float tot = n_run + k, f = __fdividef(k, tot), w = n_run * f * float(VEC / W);
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const float d = bt.mean[j] - mean[j];
+                    mean[j] += d * f;
+                    m2[j] += bt.m2[j] + d * d * w;
+                }
+                n_run = tot;
+            };
             int p = p0 + pc.r;
             for (; p + (U - 1) * pc.rp < p1; p += U * pc.rp) {
                 Pack<T, VEC> raw[U];
                 const T* at = xc + int64_t(p) * a.xp;
 #pragma unroll
                 for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * step);
-                run.template add<T, U, true>(raw, pivot, U);
+                bt.template take<U, true>(raw, pivot, U);
+                join(float(U));
             }
             if (p < p1) {
                 Pack<T, VEC> raw[U];
@@ -242,53 +411,52 @@ __global__ void __launch_bounds__(kGnThreads) gn_moments_kernel(GnPlan pl) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (u < k) raw[u] = load_pack<T, VEC>(at + u * step);
-                run.template add<T, U, false>(raw, pivot, k);
+                bt.template take<U, false>(raw, pivot, k);
+                join(float(k));
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(run.mean[j], run.m2[j]);
+            for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(mean[j], m2[j]);
         }
         __syncthreads();
-        for (int g = c0 / Cg + warp; g <= (c1 - 1) / Cg; g += kGnWarps) {
-            const int ca = max(c0, g * Cg), before = ca - g * Cg;   // channels of the group in earlier tiles
-            const int wd = (min(c1, (g + 1) * Cg) - ca) / (VEC / W), at = (ca - c0) / (VEC / W);
-            const float2 old = acc[g];
-            const float about = part[at].x;   // row 0 is there if any is
-            Merge m;
-            for (int i = lane; i < pc.rp * wd; i += 32) {
-                const int r = i / wd;
-                const float2 v = part[r * pc.nv * W + at + i - r * wd];
-                m.add(about, float((max(p1 - p0 - r, 0) + pc.rp - 1) / pc.rp) * float(VEC / W), v.x, v.y);
+        {
+            const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
+            const int lane = int(threadIdx.x) & ((1 << log) - 1), rows = p1 - p0, full = rows / pc.rp;
+            for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
+                const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
+                const bool mine = gi < gn;
+                const int ca = max(c0, g * Cg), before = ca - g * Cg;   // channels of the group in earlier tiles
+                const int wd = (min(c1, (g + 1) * Cg) - ca) / (VEC / W), at = (ca - c0) / (VEC / W);
+                const float2 old = mine ? acc[g] : make_float2(0.0f, 0.0f);
+                const float about = mine ? part[at].x : 0.0f;   // row 0 is there if any is
+                Merge m;
+                if (mine) {
+                    for (int i = lane; i < pc.rp * wd; i += 1 << log) {
+                        const int r = wd == 1 ? i : i / wd;
+                        const float2 v = part[r * pc.nv * W + at + i - r * wd];
+                        const int cnt = full + (r < rows - full * pc.rp ? 1 : 0);
+                        m.add(about, float(cnt * (VEC / W)), v.x, v.y);
+                    }
+                    if (before > 0 && lane == 0) m.add(about, float(rows) * float(before), old.x, old.y);
+                }
+                m.lanes(log);
+                __syncwarp();
+                if (mine && lane == 0) acc[g] = m.pair(about, float(rows) * float(min(c1, (g + 1) * Cg) - g * Cg));
             }
-            if (before > 0 && lane == 0) m.add(about, float(p1 - p0) * float(before), old.x, old.y);
-            m.warp();
-            if (lane == 0) acc[g] = m.pair(about);
         }
         __syncthreads();
     }
-    // one partial per cluster: its blocks share out the groups
-    cl_sync();
-    const int rank = chunk % kSweepCluster, first = chunk - rank;
     pdl_wait();   // the launches before this one are done when it is
-    for (int g = rank * kGnThreads + int(threadIdx.x); g < G; g += kSweepCluster * kGnThreads) {
-        float2 v[kSweepCluster];
-#pragma unroll
-        for (int k = 0; k < kSweepCluster; ++k) v[k] = ld_cluster_f2(cluster_map(acc + g, uint32_t(k)));
-        Merge m;
-#pragma unroll
-        for (int k = 0; k < kSweepCluster; ++k)
-            m.add(v[0].x, float(rows_of(len, first + k, pl.rows)) * float(Cg), v[k].x, v[k].y);
-        pl.moments[(int64_t(n) * (pl.parts) + first / kSweepCluster) * G + g] = m.pair(v[0].x);
-    }
-    cl_sync();    // no block leaves while a peer may read its moments
+    for (int g = threadIdx.x; g < G; g += kGnThreads)
+        pl.moments[(int64_t(n) * pl.chunks + chunk) * G + g] = acc[g];
 }
 
 // Forward, sweep 2: merges the sample's chunks, writes y.
 template <typename T, int VEC, int ACT, bool ONEG>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     float2* st = reinterpret_cast<float2*>(gn_smem);   // [G] mean, rstd
-    constexpr int NG = ONEG ? 1 : VEC, U = 4;
+    constexpr int U = 8;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
@@ -298,7 +466,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnPlan pl) {
     pdl_wait();
     {
         __shared__ Merge merged[kGnWarps][32];
-        const int parts = pl.parts, span = kSweepCluster * pl.rows;
+        const int parts = pl.chunks;
         for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the partials
             Merge m;
             const float2* from = pl.moments + int64_t(n) * parts * G + g;
@@ -307,18 +475,17 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnPlan pl) {
 #pragma unroll 8
                 for (int k = warp; k < parts; k += kGnWarps) {
                     const float2 v = from[int64_t(k) * G];
-                    m.add(about, float(rows_of(len, k, span)) * float(Cg), v.x, v.y);
+                    m.add(about, float(rows_of(len, k, pl.rows)) * float(Cg), v.x, v.y);
                 }
             merged[warp][lane] = m;
             __syncthreads();
             if (warp == 0 && g < G) {
 #pragma unroll
                 for (int k = 1; k < kGnWarps; ++k) {
-                    m.n += merged[k][lane].n;
                     m.nd += merged[k][lane].nd;
                     m.m2 += merged[k][lane].m2;
                 }
-                st[g] = mean_rstd(group_pivot(x, len, g * Cg), m.pair(about), len, Cg, a.eps);
+                st[g] = mean_rstd(group_pivot(x, len, g * Cg), m.pair(about, float(len) * float(Cg)), len, Cg, a.eps);
                 if (chunk == 0) reinterpret_cast<float2*>(a.stats)[int64_t(n) * G + g] = st[g];
             }
             __syncthreads();
@@ -330,27 +497,13 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnPlan pl) {
         const Place pc(cv, tile);
         if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
-        float mean[NG], sc[VEC], sh[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float2 v = st[(c + j) / Cg];
-            if (j < NG) mean[j] = v.x;
-            sc[j] = v.y * (a.weight ? load_param(a.weight, a.param_dtype, c + j) : 1.0f);
-            sh[j] = a.bias ? load_param(a.bias, a.param_dtype, c + j) : 0.0f;
-        }
+        Forward<T, VEC, ACT, ONEG> fw;
+        fw.load(a, c, c, Cg, st);
         auto write = [&](int p, const Pack<T, VEC>& raw) {
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                o[j] = act_fwd<ACT>((to_f32(raw.v[j]) - mean[ONEG ? 0 : j]) * sc[j] + sh[j], a.act);
-            store_pack<T, VEC>(y + int64_t(p) * C + c, pack<T, VEC>(o));
+            store_pack<T, VEC>(y + int64_t(p) * C + c, fw(raw, a.act));
         };
-        for (int p = pv + pc.r; p < pe; p += pc.rp) {   // padding
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
-            store_pack<T, VEC>(y + int64_t(p) * C + c, pack<T, VEC>(o));
-        }
+        for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
+            store_pack<T, VEC>(y + int64_t(p) * C + c, pack_zero<T, VEC>());
         int p = pv - 1 - pc.r;
         for (; p - (U - 1) * pc.rp >= p0; p -= U * pc.rp) {
             Pack<T, VEC> raw[U];
@@ -365,22 +518,20 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnPlan pl) {
 
 // Backward, sweep 1: per-channel and per-group sums over a chunk.
 template <typename T, int VEC, int ACT, bool ONEG>
-__global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
-    constexpr int NG = ONEG ? 1 : VEC, U = 4;
+    constexpr int U = 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G]
     float2* part = acc + G;                             // [rp][nv * VEC]
     const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
-    const int rank = chunk % kSweepCluster;
-    const int64_t slot = int64_t(n) * (pl.parts) + chunk / kSweepCluster;
+    const int64_t slot = int64_t(n) * pl.chunks + chunk;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
     const float2* st = reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     for (int g = threadIdx.x; g < G; g += kGnThreads) acc[g] = make_float2(0.0f, 0.0f);
     __syncthreads();
@@ -389,27 +540,13 @@ __global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(GnPlan pl) {
         const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
         if (pc.on) {
             const int c = c0 + pc.v * VEC;
-            float mean[NG], rstd[NG], w[VEC], b[VEC], sa[VEC], sb[VEC];
+            Backward<T, VEC, ACT, ONEG> bw;
+            bw.load(a, c, c, Cg, st);
+            constexpr int NP = pairs_of(VEC);
+            float2 sa[NP], sb[NP];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (j < NG) {
-                    const float2 v = st[(c + j) / Cg];
-                    mean[j] = v.x;
-                    rstd[j] = v.y;
-                }
-                w[j] = a.weight ? load_param(a.weight, a.param_dtype, c + j) : 1.0f;
-                b[j] = a.bias ? load_param(a.bias, a.param_dtype, c + j) : 0.0f;
-                sa[j] = sb[j] = 0.0f;
-            }
-            auto take = [&](const Pack<T, VEC>& rx, const Pack<T, VEC>& rg) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float xh = (to_f32(rx.v[j]) - mean[ONEG ? 0 : j]) * rstd[ONEG ? 0 : j];
-                    const float dz = to_f32(rg.v[j]) * act_slope<ACT>(xh * w[j] + b[j], a.act);
-                    sa[j] += dz;
-                    sb[j] += dz * xh;
-                }
-            };
+            for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
+            auto take = [&](const Pack<T, VEC>& rx, const Pack<T, VEC>& rg) { bw.sums(rx, rg, a.act, sa, sb); };
             int p = p0 + pc.r;
             for (; p + (U - 1) * pc.rp < p1; p += U * pc.rp) {
                 Pack<T, VEC> rx[U], rg[U];
@@ -424,7 +561,9 @@ __global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(GnPlan pl) {
             for (; p < p1; p += pc.rp)
                 take(load_pack<T, VEC>(x + int64_t(p) * a.xp + c), load_pack<T, VEC>(dy + int64_t(p) * a.gp + c));
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) part[(pc.r * pc.nv + pc.v) * VEC + j] = make_float2(sa[j], sb[j]);
+            for (int j = 0; j < VEC; ++j)
+                part[(pc.r * pc.nv + pc.v) * VEC + j] =
+                    j % 2 ? make_float2(sa[j / 2].y, sb[j / 2].y) : make_float2(sa[j / 2].x, sb[j / 2].x);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < pc.nv * VEC; i += kGnThreads) {   // rows of a channel, in order
@@ -435,57 +574,41 @@ __global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(GnPlan pl) {
                 s.y += v.y;
             }
             part[i] = s;
-        }
-        cl_sync();
-        // one partial per cluster: its blocks share out the channels
-        for (int i = rank * kGnThreads + int(threadIdx.x); i < pc.nv * VEC; i += kSweepCluster * kGnThreads) {
-            float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int k = 0; k < kSweepCluster; ++k) {
-                const float2 v = ld_cluster_f2(cluster_map(part + i, uint32_t(k)));
-                s.x += v.x;
-                s.y += v.y;
-            }
             pl.csums[slot * C + c0 + i] = s;
         }
-        for (int g = c0 / Cg + warp; g <= (c1 - 1) / Cg; g += kGnWarps) {
-            const int ca = max(c0, g * Cg), cb = min(c1, (g + 1) * Cg);
-            float2 s = make_float2(0.0f, 0.0f);
-            for (int c = ca + lane; c < cb; c += 32) {
-                const float w = a.weight ? load_param(a.weight, a.param_dtype, c) : 1.0f;
-                s.x += w * part[c - c0].x;
-                s.y += w * part[c - c0].y;
-            }
-            s.x = warp_sum<32>(s.x);
-            s.y = warp_sum<32>(s.y);
-            if (lane == 0) {
-                acc[g].x += s.x;
-                acc[g].y += s.y;
+        __syncthreads();
+        {
+            const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
+            const int lane = int(threadIdx.x) & ((1 << log) - 1);
+            for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
+                const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
+                float2 s = make_float2(0.0f, 0.0f);
+                if (gi < gn)
+                    for (int c = max(c0, g * Cg) + lane; c < min(c1, (g + 1) * Cg); c += 1 << log) {
+                        const float w = a.weight ? load_param(a.weight, a.param_dtype, c) : 1.0f;
+                        s.x += w * part[c - c0].x;
+                        s.y += w * part[c - c0].y;
+                    }
+                s = lanes_sum(s, log);
+                if (gi < gn && lane == 0) {
+                    acc[g].x += s.x;
+                    acc[g].y += s.y;
+                }
             }
         }
-        cl_sync();    // the peers have read this tile's sums
+        __syncthreads();
     }
     pdl_wait();   // the launches before this one are done when it is
-    for (int g = rank * kGnThreads + int(threadIdx.x); g < G; g += kSweepCluster * kGnThreads) {
-        float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < kSweepCluster; ++k) {
-            const float2 v = ld_cluster_f2(cluster_map(acc + g, uint32_t(k)));
-            s.x += v.x;
-            s.y += v.y;
-        }
-        pl.gsums[slot * G + g] = s;
-    }
-    cl_sync();        // no block leaves while a peer may read its sums
+    for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
 }
 
 // Backward, sweep 2: merges the sample's group sums, writes dx.
 template <typename T, int VEC, int ACT, bool ONEG>
-__global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     float4* gv = reinterpret_cast<float4*>(gn_smem);   // [G] mean, rstd, S1/m, S2/m
-    constexpr int NG = ONEG ? 1 : VEC, U = 4;
+    constexpr int U = 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
@@ -495,7 +618,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(GnPlan pl) {
     pdl_wait();
     {
         __shared__ float2 merged[kGnWarps][32];
-        const int parts = pl.parts;
+        const int parts = pl.chunks;
         for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the partials
             float2 s = make_float2(0.0f, 0.0f);
             if (g < G)
@@ -527,29 +650,16 @@ __global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(GnPlan pl) {
         const Place pc(cv, tile);
         if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
-        float w[VEC], b[VEC];
-        float4 gr[NG];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if (j < NG) gr[j] = gv[(c + j) / Cg];
-            w[j] = a.weight ? load_param(a.weight, a.param_dtype, c + j) : 1.0f;
-            b[j] = a.bias ? load_param(a.bias, a.param_dtype, c + j) : 0.0f;
-        }
+        Backward<T, VEC, ACT, ONEG> bw;
+        bw.load(a, c, c, Cg, gv);
+        PerGroup<VEC, ONEG> s1, s2;
+        s1.fill(c, Cg, [&](int g) { return gv[g].z; });
+        s2.fill(c, Cg, [&](int g) { return gv[g].w; });
         auto write = [&](int p, const Pack<T, VEC>& rx, const Pack<T, VEC>& rg) {
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float4 v = gr[ONEG ? 0 : j];
-                o[j] = dx_of<ACT>(to_f32(rx.v[j]), to_f32(rg.v[j]), v.x, v.y, w[j], b[j], make_float2(v.z, v.w), a.act);
-            }
-            store_pack<T, VEC>(dx + int64_t(p) * C + c, pack<T, VEC>(o));
+            store_pack<T, VEC>(dx + int64_t(p) * C + c, bw.dx(rx, rg, a.act, s1, s2));
         };
-        for (int p = pv + pc.r; p < pe; p += pc.rp) {   // padding
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
-            store_pack<T, VEC>(dx + int64_t(p) * C + c, pack<T, VEC>(o));
-        }
+        for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
+            store_pack<T, VEC>(dx + int64_t(p) * C + c, pack_zero<T, VEC>());
         int p = pv - 1 - pc.r;
         for (; p - (U - 1) * pc.rp >= p0; p -= U * pc.rp) {
             Pack<T, VEC> rx[U], rg[U];
@@ -594,7 +704,7 @@ struct ResPlace {
 };
 
 template <typename T, int VEC, int ACT, bool ONEG, int KV>
-__global__ void __launch_bounds__(kResThreads, 2) gn_resident_fwd_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_resident_fwd_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     const int C = int(a.C), G = int(a.G), Cg = C / G;
@@ -616,51 +726,32 @@ __global__ void __launch_bounds__(kResThreads, 2) gn_resident_fwd_kernel(GnPlan 
             ++cnt;
         }
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = int(blockDim.x) >> 5;
     if (pc.on) {
-        // two passes over the registers
-        constexpr int W = ONEG ? 1 : VEC, J = VEC / W;
-        const float inv = cnt > 0 ? 1.0f / float(cnt * J) : 0.0f;
-        float s[W], q[W], pivot[W];
+        PerGroup<VEC, ONEG> pivot;
+        pivot.fill(c, Cg, [&](int g) { return group_pivot(x - c, len, g * Cg); });
+        Batch<T, VEC, ONEG> bt;
+        bt.template take<KV, false>(raw, pivot, cnt);
+        constexpr int W = ONEG ? 1 : VEC;
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            s[j] = q[j] = 0.0f;
-            pivot[j] = group_pivot(x - c, len, (c + j) / Cg * Cg);
-        }
-#pragma unroll
-        for (int k = 0; k < KV; ++k)
-            if (k < cnt)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) s[j / J] += to_f32(raw[k].v[j]) - pivot[j / J];
-#pragma unroll
-        for (int j = 0; j < W; ++j) s[j] *= inv;
-#pragma unroll
-        for (int k = 0; k < KV; ++k) {
-            reload(raw[k]);
-            if (k < cnt)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = (to_f32(raw[k].v[j]) - pivot[j / J]) - s[j / J];
-                    q[j / J] += d * d;
-                }
-            reload(raw[k]);
-        }
-#pragma unroll
-        for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(s[j], q[j]);
+        for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(bt.mean[j], bt.m2[j]);
     }
     __syncthreads();
     {
-        const int wd = ONEG ? Cg / VEC : Cg, width = pc.nv * (ONEG ? 1 : VEC), rows = max(pv - p0, 0);
-        for (int g = warp; g < pc.gs; g += warps) {
-            const float about = part[g * wd].x;   // row 0 is there if any is
+        constexpr int J = ONEG ? VEC : 1;
+        const int wd = Cg / J, width = pc.nv * (VEC / J), rows = max(pv - p0, 0), full = rows / pc.rp;
+        const int log = lanes_log(pc.gs, int(blockDim.x)), lane = int(threadIdx.x) & ((1 << log) - 1);
+        for (int i0 = 0; i0 < pc.gs; i0 += int(blockDim.x) >> log) {
+            const int g = i0 + (int(threadIdx.x) >> log);
+            const float about = g < pc.gs ? part[g * wd].x : 0.0f;   // row 0 is there if any is
             Merge m;
-            for (int i = lane; i < pc.rp * wd; i += 32) {
-                const int r = i / wd;
-                const float2 v = part[r * width + g * wd + i - r * wd];
-                m.add(about, float((max(rows - r, 0) + pc.rp - 1) / pc.rp) * float(ONEG ? VEC : 1), v.x, v.y);
-            }
-            m.warp();
-            if (lane == 0) mine[g] = m.pair(about);
+            if (g < pc.gs)
+                for (int i = lane; i < pc.rp * wd; i += 1 << log) {
+                    const int r = wd == 1 ? i : i / wd;
+                    const float2 v = part[r * width + g * wd + i - r * wd];
+                    m.add(about, float((full + (r < rows - full * pc.rp ? 1 : 0)) * J), v.x, v.y);
+                }
+            m.lanes(log);
+            if (g < pc.gs && lane == 0) mine[g] = m.pair(about, float(rows) * float(Cg));
         }
     }
     if (pl.chunks > 1) cl_sync();
@@ -676,7 +767,7 @@ __global__ void __launch_bounds__(kResThreads, 2) gn_resident_fwd_kernel(GnPlan 
 #pragma unroll
             for (int k = 0; k < kMaxCluster; ++k)
                 if (k < pl.chunks) all.add(v[0].x, float(rows_of(len, k, pl.rows)) * float(Cg), v[k].x, v[k].y);
-            m = all.pair(v[0].x);
+            m = all.pair(v[0].x, float(len) * float(Cg));
         }
         st[g] = mean_rstd(group_pivot(x - c, len, (pc.g0 + g) * Cg), m, len, Cg, a.eps);
         if (pc.chunk == 0) reinterpret_cast<float2*>(a.stats)[int64_t(pc.n) * G + pc.g0 + g] = st[g];
@@ -684,34 +775,21 @@ __global__ void __launch_bounds__(kResThreads, 2) gn_resident_fwd_kernel(GnPlan 
     if (pl.chunks > 1) cl_arrive();   // this block has read its peers' sums
     __syncthreads();
     if (pc.on) {
-        float mean[ONEG ? 1 : VEC], sc[VEC], sh[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float2 v = st[(pc.v * VEC + j) / Cg];
-            mean[ONEG ? 0 : j] = v.x;
-            sc[j] = v.y * (a.weight ? load_param(a.weight, a.param_dtype, c + j) : 1.0f);
-            sh[j] = a.bias ? load_param(a.bias, a.param_dtype, c + j) : 0.0f;
-        }
+        Forward<T, VEC, ACT, ONEG> fw;
+        fw.load(a, c, pc.v * VEC, Cg, st);
         T* y = static_cast<T*>(a.y) + int64_t(pc.n) * a.S * C + c;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int p = p0 + pc.r + k * pc.rp;
             if (p >= pe) break;
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
-            if (k < cnt)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    o[j] = act_fwd<ACT>((to_f32(raw[k].v[j]) - mean[ONEG ? 0 : j]) * sc[j] + sh[j], a.act);
-            store_pack<T, VEC>(y + int64_t(p) * C, pack<T, VEC>(o));
+            store_pack<T, VEC>(y + int64_t(p) * C, k < cnt ? fw(raw[k], a.act) : pack_zero<T, VEC>());
         }
     }
     if (pl.chunks > 1) cl_wait();     // no block leaves while a peer may read its sums
 }
 
 template <typename T, int VEC, int ACT, bool ONEG, int KV>
-__global__ void __launch_bounds__(kResThreads, 1) gn_resident_bwd_kernel(GnPlan pl) {
+__global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     const int C = int(a.C), G = int(a.G), Cg = C / G;
@@ -735,39 +813,24 @@ __global__ void __launch_bounds__(kResThreads, 1) gn_resident_bwd_kernel(GnPlan 
             ++cnt;
         }
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = int(blockDim.x) >> 5;
     const float2* stats = reinterpret_cast<const float2*>(a.stats) + int64_t(pc.n) * G + pc.g0;
-    constexpr int NG = ONEG ? 1 : VEC;
-    float mean[NG], rstd[NG], w[VEC], b[VEC];
+    Backward<T, VEC, ACT, ONEG> bw;
     if (pc.on) {
+        bw.load(a, c, pc.v * VEC, Cg, stats);
+        constexpr int NP = pairs_of(VEC);
+        float2 sa[NP], sb[NP];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if (j < NG) {
-                const float2 v = stats[(pc.v * VEC + j) / Cg];
-                mean[j] = v.x;
-                rstd[j] = v.y;
-            }
-            w[j] = a.weight ? load_param(a.weight, a.param_dtype, c + j) : 1.0f;
-            b[j] = a.bias ? load_param(a.bias, a.param_dtype, c + j) : 0.0f;
-        }
-        float sa[VEC], sb[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sa[j] = sb[j] = 0.0f;
+        for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
-            if (k < cnt)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float xh = (to_f32(rx[k].v[j]) - mean[ONEG ? 0 : j]) * rstd[ONEG ? 0 : j];
-                    const float dz = to_f32(rg[k].v[j]) * act_slope<ACT>(xh * w[j] + b[j], a.act);
-                    sa[j] += dz;
-                    sb[j] += dz * xh;
-                }
+            if (k < cnt) bw.sums(rx[k], rg[k], a.act, sa, sb);
             reload(rx[k]);
             reload(rg[k]);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) part[(pc.r * pc.nv + pc.v) * VEC + j] = make_float2(sa[j], sb[j]);
+        for (int j = 0; j < VEC; ++j)
+            part[(pc.r * pc.nv + pc.v) * VEC + j] =
+                j % 2 ? make_float2(sa[j / 2].y, sb[j / 2].y) : make_float2(sa[j / 2].x, sb[j / 2].x);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < pc.nv * VEC; i += blockDim.x) {   // rows of a channel, in order
@@ -778,19 +841,23 @@ __global__ void __launch_bounds__(kResThreads, 1) gn_resident_bwd_kernel(GnPlan 
             s.y += v.y;
         }
         part[i] = s;
-        pl.csums[(int64_t(pc.n) * pl.parts + pc.chunk) * C + pc.c0 + i] = s;
+        pl.csums[(int64_t(pc.n) * pl.chunks + pc.chunk) * C + pc.c0 + i] = s;
     }
     __syncthreads();
-    for (int g = warp; g < pc.gs; g += warps) {
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int i = g * Cg + lane; i < (g + 1) * Cg; i += 32) {
-            const float wi = a.weight ? load_param(a.weight, a.param_dtype, pc.c0 + i) : 1.0f;
-            s.x += wi * part[i].x;
-            s.y += wi * part[i].y;
+    {
+        const int log = lanes_log(pc.gs, int(blockDim.x)), lane = int(threadIdx.x) & ((1 << log) - 1);
+        for (int i0 = 0; i0 < pc.gs; i0 += int(blockDim.x) >> log) {
+            const int g = i0 + (int(threadIdx.x) >> log);
+            float2 s = make_float2(0.0f, 0.0f);
+            if (g < pc.gs)
+                for (int i = g * Cg + lane; i < (g + 1) * Cg; i += 1 << log) {
+                    const float w = a.weight ? load_param(a.weight, a.param_dtype, pc.c0 + i) : 1.0f;
+                    s.x += w * part[i].x;
+                    s.y += w * part[i].y;
+                }
+            s = lanes_sum(s, log);
+            if (g < pc.gs && lane == 0) mine[g] = s;
         }
-        s.x = warp_sum<32>(s.x);
-        s.y = warp_sum<32>(s.y);
-        if (lane == 0) mine[g] = s;
     }
     if (pl.chunks > 1) cl_sync();
     else __syncthreads();
@@ -813,22 +880,15 @@ __global__ void __launch_bounds__(kResThreads, 1) gn_resident_bwd_kernel(GnPlan 
     __syncthreads();
     if (pc.on && a.dx != nullptr) {
         T* dx = static_cast<T*>(a.dx) + int64_t(pc.n) * a.S * C + c;
-        float2 sg[NG];
-#pragma unroll
-        for (int j = 0; j < NG; ++j) sg[j] = sums[(pc.v * VEC + j) / Cg];
+        PerGroup<VEC, ONEG> s1, s2;
+        s1.fill(pc.v * VEC, Cg, [&](int g) { return sums[g].x; });
+        s2.fill(pc.v * VEC, Cg, [&](int g) { return sums[g].y; });
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int p = p0 + pc.r + k * pc.rp;
             if (p >= pe) break;
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
-            if (k < cnt)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    o[j] = dx_of<ACT>(to_f32(rx[k].v[j]), to_f32(rg[k].v[j]), mean[ONEG ? 0 : j], rstd[ONEG ? 0 : j],
-                                      w[j], b[j], sg[ONEG ? 0 : j], a.act);
-            store_pack<T, VEC>(dx + int64_t(p) * C, pack<T, VEC>(o));
+            store_pack<T, VEC>(dx + int64_t(p) * C,
+                               k < cnt ? bw.dx(rx[k], rg[k], a.act, s1, s2) : pack_zero<T, VEC>());
         }
     }
     if (pl.chunks > 1) cl_wait();     // no block leaves while a peer may read its sums
@@ -846,19 +906,18 @@ void sweep_plan(GnPlan& pl, int esz, bool backward, int& batch) {
     int64_t nb = kBatchBytes / (bytes > 0 ? bytes : 1);
     nb = nb < 1 ? 1 : nb > a.N ? a.N : nb;
     nb = ceil_div(a.N, ceil_div(a.N, nb));   // batches of one size
-    // about four blocks per SM over a batch, at least 32 positions each
-    int64_t want = ceil_div(int64_t(148) * 4, nb);
+    // one block per SM over a batch, at least 32 positions each
+    int64_t want = kSMs / nb < 1 ? 1 : kSMs / nb;
     if (want > ceil_div(a.S, 32)) want = ceil_div(a.S, 32);
     batch = int(nb);
-    pl.parts = int(ceil_div(want, kSweepCluster));
-    pl.chunks = pl.parts * kSweepCluster;
-    pl.rows = int(ceil_div(a.S, pl.chunks));   // the last chunks may be empty
+    pl.rows = int(ceil_div(a.S, want));
+    pl.chunks = int(ceil_div(a.S, pl.rows));
 }
 
 size_t carve(void* ws, GnPlan& pl, bool backward) {
     const GroupNormArgs& a = pl.a;
     Carve cv(ws);
-    const size_t blocks = size_t(a.N) * size_t(pl.parts);
+    const size_t blocks = size_t(a.N) * size_t(pl.chunks);
     if (!backward) {
         pl.moments = cv.take<float2>(blocks * size_t(a.G));
     } else {
@@ -882,7 +941,7 @@ size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward
         const size_t b = carve(nullptr, pl, backward);
         if (b > most) most = b;
     }
-    pl.parts = kMaxCluster;   // resident: one of each block
+    pl.chunks = kMaxCluster;   // resident
     const size_t b = backward ? carve(nullptr, pl, true) : 0;
     return b > most ? b : most;
 }
@@ -926,31 +985,32 @@ int launch_params(const GnPlan& pl, cudaStream_t st) {
     return launch(gn_params_kernel, pl, ceil_div(pl.a.C, 32), kGnThreads, 0, 1, false, st);
 }
 
-// The resident plan of a problem, if a cluster holds a slab of it.
+// The resident plan of a problem, if its blocks hold it in registers all at
+// once, one block per SM.
 //
 // The slab is the narrowest run of whole groups of at least 64 bytes (two DRAM
 // sectors, so neighbouring slabs share no sector pair) whose width is a whole
 // number of vectors; blocks are added to a cluster until its registers hold
-// the sample's positions, and beyond that (up to 8) while all blocks together
-// stay within two per SM, since a smaller share per block is a shorter call.
-bool resident_plan(GnPlan& pl, int vec, int esz, int& threads, int& vecs) {
+// the sample's positions, and beyond that (up to 8) while every block has an
+// SM of its own, since a smaller share per block is a shorter call.
+bool resident_plan(GnPlan& pl, int vec, int esz, bool backward, int& threads, int& vecs) {
     const GroupNormArgs& a = pl.a;
     const int64_t Cg = a.C / a.G;
     int64_t gs = 1;
     while (gs < a.G && (gs * Cg * esz < 64 || (gs * Cg) % vec != 0)) ++gs;
     const int64_t nv = gs * Cg / vec;
-    if ((gs * Cg) % vec != 0 || nv > kResThreads) return false;
-    const int64_t rp = kResThreads / nv, slabs = ceil_div(a.G, gs);
-    int64_t K = ceil_div(a.S, rp * res_vecs(vec * esz));
-    if (K > kMaxCluster) return false;
-    while (2 * K <= kMaxCluster && a.N * slabs * 2 * K <= 2 * 148 && ceil_div(a.S, 2 * K) >= rp) K *= 2;
+    if ((gs * Cg) % vec != 0 || nv > kGnThreads) return false;
+    const int64_t rp = kGnThreads / nv, slabs = ceil_div(a.G, gs);
+    int64_t K = ceil_div(a.S, rp * res_vecs(vec * esz, backward));
+    if (K > kMaxCluster || a.N * slabs * K > kSMs) return false;
+    while (2 * K <= kMaxCluster && a.N * slabs * 2 * K <= kSMs && ceil_div(a.S, 2 * K) >= rp) K *= 2;
     const int64_t rows = ceil_div(a.S, K);
     K = ceil_div(a.S, rows);
-    pl.chunks = pl.parts = int(K);
+    pl.chunks = int(K);
     pl.rows = int(rows);
     pl.slab_groups = int(gs);
     pl.slabs = int(slabs);
-    threads = kResThreads;
+    threads = kGnThreads;
     while (threads > 128 && (threads / 2) / nv >= rows) threads /= 2;   // one vector a thread is enough
     vecs = int(ceil_div(rows, threads / nv));
     return true;
@@ -965,9 +1025,9 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
         ProfScope ps(DOT_K_NORM_FWD, st);
         return launch(gn_resident_fwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, false, st);
     }
-    carve(ws, pl, true);
-    int rc;
-    {
+    int rc = DOT_OK;
+    if constexpr (KV <= res_vecs(VEC * sizeof(T), true)) {
+        carve(ws, pl, true);
         ProfScope ps(DOT_K_NORM_BWD, st);
         rc = launch(gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, false, st);
     }
@@ -989,8 +1049,8 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
         const bool second = !backward || a.dx != nullptr;
         ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st, second ? 2 : 1);
         int rc = backward
-            ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, kSweepCluster, n > 0, st)
-            : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, kSweepCluster, n > 0, st);
+            ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, n > 0, st)
+            : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, n > 0, st);
         if (!rc && second)
             rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st)
                           : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st);
@@ -1004,11 +1064,12 @@ int run(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st) {
     GnPlan pl{};
     pl.a = a;
     int threads, vecs;
-    if (!resident_plan(pl, VEC, sizeof(T), threads, vecs)) return sweep_run<T, VEC, ACT, ONEG>(pl, ws, backward, st);
-    constexpr int most = res_vecs(VEC * sizeof(T)), some = most / 2;
-    if (vecs == 1 && VEC * sizeof(T) == 16) return resident_run<T, VEC, ACT, ONEG, 1>(pl, ws, threads, backward, st);
-    if (vecs <= some) return resident_run<T, VEC, ACT, ONEG, some>(pl, ws, threads, backward, st);
-    return resident_run<T, VEC, ACT, ONEG, most>(pl, ws, threads, backward, st);
+    if (!resident_plan(pl, VEC, sizeof(T), backward, threads, vecs))
+        return sweep_run<T, VEC, ACT, ONEG>(pl, ws, backward, st);
+    constexpr int most = res_vecs(VEC * sizeof(T), true);
+    if (vecs <= most / 4) return resident_run<T, VEC, ACT, ONEG, most / 4>(pl, ws, threads, backward, st);
+    if (vecs <= most) return resident_run<T, VEC, ACT, ONEG, most>(pl, ws, threads, backward, st);
+    return resident_run<T, VEC, ACT, ONEG, res_vecs(VEC * sizeof(T), false)>(pl, ws, threads, false, st);
 }
 
 template <typename T, int VEC, int ACT>

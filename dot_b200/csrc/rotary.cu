@@ -98,27 +98,25 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a, RotPl
                 continue;
             }
             const Pack<T, VP> p1 = load_pack<T, VP>(src + o1);
-            float e[2 * VP], u[VP], v[VP];
+            float e[2 * VP];
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
                 e[j] = to_f32(p0.v[j]);
                 e[VP + j] = to_f32(p1.v[j]);
             }
-            float r[2 * VP];
+            Pack<T, VP> r0, r1;
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
                 const float x = IL ? e[2 * j] : e[j], y = IL ? e[2 * j + 1] : e[VP + j];
                 // the products' roundings are spelled out: every width gives the same bits
-                r[IL ? 2 * j : j] = __fmaf_rn(x, c[j], -__fmul_rn(y, s[j]));
-                r[IL ? 2 * j + 1 : VP + j] = __fmaf_rn(y, c[j], __fmul_rn(x, s[j]));
+                const T u = from_f32<T>(__fmaf_rn(x, c[j], -__fmul_rn(y, s[j])));
+                const T v = from_f32<T>(__fmaf_rn(y, c[j], __fmul_rn(x, s[j])));
+                const int iu = IL ? 2 * j : j, iv = IL ? 2 * j + 1 : VP + j;
+                (iu < VP ? r0.v[iu % VP] : r1.v[iu % VP]) = u;
+                (iv < VP ? r0.v[iv % VP] : r1.v[iv % VP]) = v;
             }
-#pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                u[j] = r[j];
-                v[j] = r[VP + j];
-            }
-            store_pack<T, VP>(dst + o0, pack<T, VP>(u));
-            store_pack<T, VP>(dst + o1, pack<T, VP>(v));
+            store_pack<T, VP>(dst + o0, r0);
+            store_pack<T, VP>(dst + o1, r1);
         }
     }
 }
