@@ -127,7 +127,8 @@ int dot_rotary(const void* q, const int64_t* q_strides, int64_t Hq, const void* 
     if (pos_dtype != DOT_F32 && pos_dtype != DOT_I32 && pos_dtype != DOT_I64)
         return fail(DOT_ERR_UNSUPPORTED, "positions must be int32, int64 or float32");
     if (P > kMaxPairs) return fail(DOT_ERR_UNSUPPORTED, "more than 4096 pairs in a head");
-    if (B > 0x7fffffff || L > 0x7fffffff || Hq + Hk > 0x7fffff) return fail(DOT_ERR_UNSUPPORTED, "dimension too large");
+    // a block's tokens are counted past the end of a sample in 31 bits
+    if (B > 0x7fffffff || L > 0x7fffff00 || Hq + Hk > 0x7fffff) return fail(DOT_ERR_UNSUPPORTED, "dimension too large");
     if (B == 0 || L == 0 || D == 0 || Hq + Hk == 0) return DOT_OK;
     if ((Hq > 0 && (!q || !q_out || !q_strides)) || (Hk > 0 && (!k || !k_out || !k_strides)) || !positions ||
         !pos_strides || (P > 0 && !freqs))

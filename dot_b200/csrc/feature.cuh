@@ -17,6 +17,21 @@
 
 namespace dotb {
 
+// Division by a number that the host knows: n / d = (n * m) >> 32 >> s for
+// n < 2^31 (Granlund and Montgomery, 1994), two instructions.
+struct FastDiv {
+    uint32_t d = 1, m = 0, s = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        if (d > 1) {
+            while ((1ull << s) < d) ++s;                          // ceil(log2 d)
+            m = uint32_t(((1ull << 31 << s) + d - 1) / d);        // ceil(2^(31+s) / d) < 2^32
+            --s;
+        }
+    }
+    __device__ __forceinline__ int div(int n) const { return d == 1 ? n : int(__umulhi(uint32_t(n), m) >> s); }
+};
+
 // N elements of T as one naturally aligned access (1 to 16 bytes).
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Pack {

@@ -25,6 +25,7 @@ struct RotPlan {
     int hgroups;        // heads of a token handled side by side
     int tokens;         // tokens per block
     int64_t ntok;       // B * L
+    FastDiv by_slots, by_token, by_pairs, by_axes, by_len;   // slots, slots * hgroups, P, A, L
 };
 
 template <typename I>
@@ -32,91 +33,168 @@ __device__ __forceinline__ double position(const void* p, int64_t i) {
     return double(static_cast<const I*>(p)[i]);
 }
 
-// Sine and cosine of a token's angle.  The angle in turns is formed in fp64
-// and reduced to [-1/2, 1/2] before it is rounded to fp32: a position of 2^30
-// keeps an absolute error below 2^-20 turns where an fp32 angle has lost it.
-template <typename PT>
-__device__ __forceinline__ float2 sincos_of(const RotaryArgs& a, int64_t pos_off, int p) {
-    double angle = 0.0;
-    for (int ax = 0; ax < a.A; ++ax)
-        angle = fma(position<PT>(a.positions, pos_off + ax * a.ps[2]), double(a.freqs[p * a.A + ax]), angle);
-    const double turns = angle * 0.15915494309189533577;   // 1 / (2 pi)
+// Cosine and sine of an angle given in turns, in fp64: reduced to [-1/2, 1/2]
+// before it is rounded to fp32, so a position of 2^30 keeps an absolute error
+// below 2^-20 turns where an fp32 angle has lost it.  16-bit results take the
+// SFU's sine and cosine (absolute error 2^-21 within half a turn, a thousandth
+// of their rounding), float32 the accurate ones.
+template <typename T>
+__device__ __forceinline__ float2 cos_sin(double turns) {
     const float r = float(turns - rint(turns));
     float s, c;
-    sincospif(2.0f * r, &s, &c);
-    return make_float2(c, a.inverse ? -s : s);
+    if constexpr (sizeof(T) == 2) {
+        const float x = r * 6.2831853f;
+        s = __sinf(x);
+        c = __cosf(x);
+    } else {
+        sincospif(2.0f * r, &s, &c);
+    }
+    return make_float2(c, s);
 }
 
+// A vector of VP pairs of one head, turned: (x, y) -> (x c - y s, y c + x s).
+// The roundings are the same at every width: a product, then an fma.
+template <typename T, int VP, bool IL>
+struct Turn {
+    static constexpr int NP = pairs_of(VP);
+    float2 c[IL ? VP : NP], s[IL ? VP : NP], ns[IL ? 1 : NP];
+    __device__ __forceinline__ void load(const float2* cs) {
+        if constexpr (IL) {
+#pragma unroll
+            for (int j = 0; j < VP; ++j) {
+                c[j] = splat2(cs[j].x);
+                s[j] = make_float2(-cs[j].y, cs[j].y);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const float2 u = cs[2 * j], v = VP == 1 ? u : cs[2 * j + 1];
+                c[j] = make_float2(u.x, v.x);
+                s[j] = make_float2(u.y, v.y);
+                ns[j] = make_float2(-u.y, -v.y);
+            }
+        }
+    }
+    // p0, p1: the pairs' first and second elements, or with IL the 2 VP elements in order
+    __device__ __forceinline__ void operator()(Pack<T, VP>& p0, Pack<T, VP>& p1) const {
+        if constexpr (IL && VP == 1) {
+            const float2 e = make_float2(to_f32(p0.v[0]), to_f32(p1.v[0]));
+            const float2 r = fma2(e, c[0], mul2(make_float2(e.y, e.x), s[0]));
+            p0.v[0] = from_f32<T>(r.x);
+            p1.v[0] = from_f32<T>(r.y);
+        } else {
+            float2 x[NP], y[NP];
+            unpack(p0, x);
+            unpack(p1, y);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                if constexpr (IL) {
+                    x[j] = fma2(x[j], c[j], mul2(make_float2(x[j].y, x[j].x), s[j]));
+                    y[j] = fma2(y[j], c[NP + j], mul2(make_float2(y[j].y, y[j].x), s[NP + j]));
+                } else {
+                    const float2 u = fma2(x[j], c[j], mul2(y[j], ns[j]));
+                    y[j] = fma2(y[j], c[j], mul2(x[j], s[j]));
+                    x[j] = u;
+                }
+            }
+            p0 = pack<T, VP>(x);
+            p1 = pack<T, VP>(y);
+        }
+    }
+};
+
 template <typename T, int VP, bool IL, typename PT>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a, RotPlan pl) {
-    extern __shared__ float2 cs[];   // [tokens][P] cos, sin
-    const int P = int(a.P);
+__global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(RotaryArgs a, RotPlan pl) {
+    extern __shared__ double rot_smem[];
+    const int P = int(a.P), A = a.A;
+    double* pos = rot_smem;                                            // [tokens][A] positions in turns
+    float2* cs = reinterpret_cast<float2*>(pos + pl.tokens * A);       // [tokens][P] cos, sin
     const int64_t t0 = int64_t(blockIdx.x) * pl.tokens;
     const int nt = int(min(int64_t(pl.tokens), pl.ntok - t0));
-    for (int i = threadIdx.x; i < nt * P; i += kRotThreads) {
-        const int tl = i / P, p = i - tl * P;
-        const int64_t t = t0 + tl, b = t / a.L, l = t - b * a.L;
-        cs[i] = sincos_of<PT>(a, b * a.ps[0] + l * a.ps[1], p);
+    const int64_t b0 = pl.ntok <= 0x7fffffff ? int64_t(pl.by_len.div(int(t0))) : t0 / a.L;
+    const int l0 = int(t0 - b0 * a.L);   // and at most 256 tokens on: below 2^31
+
+    // a thread's vectors: token tl, the head group's first head hg, the offsets
+    // of its two vectors within a head
+    constexpr int U = 4;   // heads in flight
+    const int work = nt * pl.slots * pl.hgroups;
+    const int Hq = int(a.Hq), H = Hq + int(a.Hk);
+    int tl, hg, o0, o1;
+    bool turn, second;
+    int slot;
+    const T *q, *k;
+    auto place = [&](int i) {
+        tl = pl.by_token.div(i);
+        const int w = i - tl * (pl.slots * pl.hgroups);
+        hg = pl.by_slots.div(w);
+        slot = w - hg * pl.slots;
+        turn = slot < pl.pair_slots;
+        o0 = turn ? (IL ? slot * 2 * VP : slot * VP) : 2 * P + (slot - pl.pair_slots) * 2 * VP;
+        o1 = turn && !IL ? P + o0 : o0 + VP;
+        second = turn || o1 < int(a.D);
+        const int db = pl.by_len.div(l0 + tl);
+        const int64_t b = b0 + db, l = l0 + tl - db * int(a.L);
+        q = static_cast<const T*>(a.q) + b * a.qs[0] + l * a.qs[1];
+        k = static_cast<const T*>(a.k) + b * a.ks[0] + l * a.ks[1];
+    };
+    Pack<T, VP> p0[U], p1[U];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * pl.hgroups;
+            if (h < H) {
+                const T* src = h < Hq ? q + h * a.qs[2] : k + (h - Hq) * a.ks[2];
+                p0[u] = load_pack<T, VP>(src + o0);
+                if (second) p1[u] = load_pack<T, VP>(src + o1);
+            }
+        }
+    };
+    int i = threadIdx.x;
+    if (i < work) {
+        place(i);
+        fetch(hg);   // on their way while the angles are formed
+    }
+
+    for (int j = threadIdx.x; j < nt * A; j += kRotThreads) {
+        const int tk = pl.by_axes.div(j), ax = j - tk * A;
+        const int db = pl.by_len.div(l0 + tk), l = l0 + tk - db * int(a.L);
+        pos[j] = position<PT>(a.positions, (b0 + db) * a.ps[0] + l * a.ps[1] + ax * a.ps[2]) *
+                 0.15915494309189533577;   // 1 / (2 pi)
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < nt * P; j += kRotThreads) {
+        const int tk = pl.by_pairs.div(j), p = j - tk * P;
+        double turns = 0.0;
+        for (int ax = 0; ax < A; ++ax) turns = fma(pos[tk * A + ax], double(a.freqs[p * A + ax]), turns);
+        const float2 v = cos_sin<T>(turns);
+        cs[j] = make_float2(v.x, a.inverse ? -v.y : v.y);
     }
     __syncthreads();
 
-    const int per_token = pl.slots * pl.hgroups;
-    const int H = int(a.Hq + a.Hk);
-    for (int i = threadIdx.x; i < nt * per_token; i += kRotThreads) {
-        const int tl = i / per_token, w = i - tl * per_token;
-        const int hg = w / pl.slots, slot = w - hg * pl.slots;
-        const int64_t t = t0 + tl, b = t / a.L, l = t - b * a.L;
-        const bool turn = slot < pl.pair_slots;
-        float c[VP], s[VP];
-        int o0, o1;          // offsets of the slot's two vectors within a head
-        bool second = true;
-        if (turn) {
-#pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                const float2 v = cs[tl * P + slot * VP + j];
-                c[j] = v.x;
-                s[j] = v.y;
-            }
-            o0 = IL ? slot * 2 * VP : slot * VP;
-            o1 = IL ? o0 + VP : P + o0;
-        } else {
-            o0 = 2 * P + (slot - pl.pair_slots) * 2 * VP;
-            o1 = o0 + VP;
-            second = o1 < int(a.D);
+    for (; i < work; i += kRotThreads) {
+        if (i >= kRotThreads) {
+            place(i);
+            fetch(hg);
         }
-        for (int h = hg; h < H; h += pl.hgroups) {
-            const bool is_q = h < int(a.Hq);
-            const int hh = is_q ? h : h - int(a.Hq);
-            const T* src = is_q ? static_cast<const T*>(a.q) + b * a.qs[0] + l * a.qs[1] + hh * a.qs[2]
-                                : static_cast<const T*>(a.k) + b * a.ks[0] + l * a.ks[1] + hh * a.ks[2];
-            T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.Hq + hh) * a.D
-                          : static_cast<T*>(a.k_out) + (t * a.Hk + hh) * a.D;
-            const Pack<T, VP> p0 = load_pack<T, VP>(src + o0);
-            if (!turn) {
-                store_pack<T, VP>(dst + o0, p0);
-                if (second) store_pack<T, VP>(dst + o1, load_pack<T, VP>(src + o1));
-                continue;
-            }
-            const Pack<T, VP> p1 = load_pack<T, VP>(src + o1);
-            float e[2 * VP];
+        Turn<T, VP, IL> tn;
+        if (turn) tn.load(cs + tl * P + slot * VP);
+        const int64_t t = t0 + tl;
+        T* qo = static_cast<T*>(a.q_out) + t * a.Hq * a.D;
+        T* ko = static_cast<T*>(a.k_out) + t * a.Hk * a.D;
+        for (int h0 = hg;;) {
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                e[j] = to_f32(p0.v[j]);
-                e[VP + j] = to_f32(p1.v[j]);
+            for (int u = 0; u < U; ++u) {
+                const int h = h0 + u * pl.hgroups;
+                if (h < H) {
+                    T* dst = h < Hq ? qo + int64_t(h) * a.D : ko + int64_t(h - Hq) * a.D;
+                    if (turn) tn(p0[u], p1[u]);
+                    store_pack<T, VP>(dst + o0, p0[u]);
+                    if (second) store_pack<T, VP>(dst + o1, p1[u]);
+                }
             }
-            Pack<T, VP> r0, r1;
-#pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                const float x = IL ? e[2 * j] : e[j], y = IL ? e[2 * j + 1] : e[VP + j];
-                // the products' roundings are spelled out: every width gives the same bits
-                const T u = from_f32<T>(__fmaf_rn(x, c[j], -__fmul_rn(y, s[j])));
-                const T v = from_f32<T>(__fmaf_rn(y, c[j], __fmul_rn(x, s[j])));
-                const int iu = IL ? 2 * j : j, iv = IL ? 2 * j + 1 : VP + j;
-                (iu < VP ? r0.v[iu % VP] : r1.v[iu % VP]) = u;
-                (iv < VP ? r0.v[iv % VP] : r1.v[iv % VP]) = v;
-            }
-            store_pack<T, VP>(dst + o0, r0);
-            store_pack<T, VP>(dst + o1, r1);
+            h0 += U * pl.hgroups;
+            if (h0 >= H) break;
+            fetch(h0);
         }
     }
 }
@@ -129,20 +207,24 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
     pl.slots = pl.pair_slots + int(ceil_div(ceil_div(a.D - 2 * a.P, VP), 2));
     const int64_t H = a.Hq + a.Hk;
     // Heads side by side: all of them for a few tokens (one access each, so a
-    // small call is one round trip), fewer as the tokens alone fill the GPU.
-    int64_t hg = H;
-    while (hg > 1 && pl.ntok * pl.slots * hg > int64_t(148) * 2048 * 4) hg = (hg + 1) / 2;
-    pl.hgroups = int(hg);
+    // small call is one round trip); four to a thread, loaded together, where
+    // that alone fills the GPU.
+    pl.hgroups = int(pl.ntok * pl.slots * H <= int64_t(148) * 2048 ? H : ceil_div(H, 4));
     const int64_t per_token = int64_t(pl.slots) * pl.hgroups;
     int64_t tokens = per_token >= kRotThreads ? 1 : kRotThreads / per_token;
     const int64_t fit = a.P > 0 ? kMaxPairs / a.P : tokens;
     if (tokens > fit) tokens = fit;
     pl.tokens = int(tokens);
+    pl.by_slots = FastDiv(uint32_t(pl.slots));
+    pl.by_token = FastDiv(uint32_t(per_token));
+    pl.by_pairs = FastDiv(uint32_t(a.P > 0 ? a.P : 1));
+    pl.by_axes = FastDiv(uint32_t(a.A));
+    pl.by_len = FastDiv(uint32_t(a.L));
     const int64_t blocks = ceil_div(pl.ntok, tokens);
     if (blocks > 0x7fffffff) return fail(DOT_ERR_UNSUPPORTED, "too many tokens");
     ProfScope ps(DOT_K_ROTARY, st);
     rotary_kernel<T, VP, IL, PT>
-        <<<unsigned(blocks), kRotThreads, size_t(tokens) * size_t(a.P) * sizeof(float2), st>>>(a, pl);
+        <<<unsigned(blocks), kRotThreads, size_t(tokens) * size_t(a.P + a.A) * 8, st>>>(a, pl);
     return check_launch("rotary");
 }
 
