@@ -124,6 +124,12 @@ def stream_of(t: torch.Tensor):
     return _vp(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(device_index: int) -> int:
+    """The current stream of a device as an address (``stream_of`` without building a Stream object:
+    2 us less of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def workspace(nbytes: int, device) -> torch.Tensor | None:
     if nbytes <= 0:
         return None

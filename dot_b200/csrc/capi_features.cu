@@ -1,9 +1,9 @@
 // extern "C" boundary of the feature operators (declared in
-// include/dot_b200.h): argument checks, then the launchers of features.h.
+// include/dot_b200.h): argument checks, then the launchers of feature_ops.h.
 #include <cmath>
 #include <string>
 
-#include "features.h"
+#include "feature_ops.h"
 #include "internal.h"
 
 using namespace dotb;

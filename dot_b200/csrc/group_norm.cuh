@@ -26,7 +26,7 @@
 
 #include "cluster.cuh"
 #include "feature.cuh"
-#include "features.h"
+#include "feature_ops.h"
 #include "internal.h"
 #include "tma.cuh"
 

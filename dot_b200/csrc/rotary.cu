@@ -7,25 +7,38 @@
 // orthogonal.  Bound: memory (each element is read and written once, with
 // about five operations); a token's P sines and cosines serve all its heads.
 //
-// A block takes kRotThreads threads' worth of whole tokens: it forms their
-// sines and cosines once into shared memory, then every thread owns one
-// vector of VP pairs of a token (kept in registers) and walks the heads.
+// A block takes a few whole tokens.  Each thread owns one vector of VP pairs of
+// a token over a run of heads and issues its first loads; while they are on
+// their way the block forms the tokens' sines and cosines, once, in shared
+// memory; then the thread keeps its own in registers and turns its heads.
 #include "feature.cuh"
-#include "features.h"
+#include "feature_ops.h"
 #include "internal.h"
 
 namespace dotb {
 namespace {
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
+constexpr int kRotRun = 4;      // consecutive heads of a thread in a large call
+
+// Heads that a thread loads together, and blocks per SM.  Small blocks, so that
+// one block's angles overlap another's copies.  Measured on 98 MB of bfloat16
+// and 32 MB of float32 (both read and written): 4 heads and 5 blocks 35.9 and
+// 15.3 us, 2 and 8 38.2 and 13.9, 4 and 4 38.3 and 15.4; blocks of 256 threads
+// 40.1 and 16.2.
+template <typename T>
+constexpr int rot_heads() { return sizeof(T) == 2 ? 4 : 2; }
+template <typename T>
+constexpr int rot_blocks() { return sizeof(T) == 2 ? 5 : 8; }
 
 struct RotPlan {
     int slots;          // threads per head: P / VP pair vectors, then the copied tail's vectors (two per slot)
     int pair_slots;
-    int hgroups;        // heads of a token handled side by side
+    int run;            // consecutive heads of a thread
+    int q_runs, runs;   // runs of q, and of q and k, that a token is split into
     int tokens;         // tokens per block
     int64_t ntok;       // B * L
-    FastDiv by_slots, by_token, by_pairs, by_axes, by_len;   // slots, slots * hgroups, P, A, L
+    FastDiv by_slots, by_token, by_pairs, by_axes, by_len;   // slots, slots * runs, P, A, L
 };
 
 template <typename I>
@@ -104,7 +117,7 @@ struct Turn {
 };
 
 template <typename T, int VP, bool IL, typename PT>
-__global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(RotaryArgs a, RotPlan pl) {
+__global__ void __launch_bounds__(kRotThreads, rot_blocks<T>()) rotary_kernel(RotaryArgs a, RotPlan pl) {
     extern __shared__ double rot_smem[];
     const int P = int(a.P), A = a.A;
     double* pos = rot_smem;                                            // [tokens][A] positions in turns
@@ -114,45 +127,49 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(RotaryArgs a, Ro
     const int64_t b0 = pl.ntok <= 0x7fffffff ? int64_t(pl.by_len.div(int(t0))) : t0 / a.L;
     const int l0 = int(t0 - b0 * a.L);   // and at most 256 tokens on: below 2^31
 
-    // a thread's vectors: token tl, the head group's first head hg, the offsets
-    // of its two vectors within a head
-    constexpr int U = 4;   // heads in flight
-    const int work = nt * pl.slots * pl.hgroups;
-    const int Hq = int(a.Hq), H = Hq + int(a.Hk);
-    int tl, hg, o0, o1;
+    // A thread's work: token tl, `heads` consecutive heads of q or of k, and the
+    // offsets o0, o1 of its two vectors within a head.
+    constexpr int U = rot_heads<T>();
+    const int work = nt * pl.slots * pl.runs;
+    int tl, slot, heads;
+    int64_t o1, stride;        // o1 counted from o0
     bool turn, second;
-    int slot;
-    const T *q, *k;
+    const T* src;
+    T* dst;
     auto place = [&](int i) {
         tl = pl.by_token.div(i);
-        const int w = i - tl * (pl.slots * pl.hgroups);
-        hg = pl.by_slots.div(w);
-        slot = w - hg * pl.slots;
+        const int w = i - tl * (pl.slots * pl.runs);
+        const int run = pl.by_slots.div(w);
+        slot = w - run * pl.slots;
         turn = slot < pl.pair_slots;
-        o0 = turn ? (IL ? slot * 2 * VP : slot * VP) : 2 * P + (slot - pl.pair_slots) * 2 * VP;
-        o1 = turn && !IL ? P + o0 : o0 + VP;
-        second = turn || o1 < int(a.D);
+        const int o0 = turn ? (IL ? slot * 2 * VP : slot * VP) : 2 * P + (slot - pl.pair_slots) * 2 * VP;
+        o1 = turn && !IL ? P : VP;
+        second = turn || o0 + VP < int(a.D);
         const int db = pl.by_len.div(l0 + tl);
-        const int64_t b = b0 + db, l = l0 + tl - db * int(a.L);
-        q = static_cast<const T*>(a.q) + b * a.qs[0] + l * a.qs[1];
-        k = static_cast<const T*>(a.k) + b * a.ks[0] + l * a.ks[1];
+        const int64_t b = b0 + db, l = l0 + tl - db * int(a.L), t = t0 + tl;
+        const bool is_q = run < pl.q_runs;
+        const int h0 = (is_q ? run : run - pl.q_runs) * pl.run;
+        const int64_t H = is_q ? a.Hq : a.Hk;
+        heads = min(pl.run, int(H) - h0);
+        stride = is_q ? a.qs[2] : a.ks[2];
+        src = is_q ? static_cast<const T*>(a.q) + b * a.qs[0] + l * a.qs[1]
+                   : static_cast<const T*>(a.k) + b * a.ks[0] + l * a.ks[1];
+        src += h0 * stride + o0;
+        dst = static_cast<T*>(is_q ? a.q_out : a.k_out) + (t * H + h0) * a.D + o0;
     };
     Pack<T, VP> p0[U], p1[U];
-    auto fetch = [&](int h0) {
+    auto fetch = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + u * pl.hgroups;
-            if (h < H) {
-                const T* src = h < Hq ? q + h * a.qs[2] : k + (h - Hq) * a.ks[2];
-                p0[u] = load_pack<T, VP>(src + o0);
-                if (second) p1[u] = load_pack<T, VP>(src + o1);
+        for (int u = 0; u < U; ++u)
+            if (u < heads) {
+                p0[u] = load_pack<T, VP>(src + u * stride);
+                if (second) p1[u] = load_pack<T, VP>(src + u * stride + o1);
             }
-        }
     };
     int i = threadIdx.x;
     if (i < work) {
         place(i);
-        fetch(hg);   // on their way while the angles are formed
+        fetch();   // on their way while the angles are formed
     }
 
     for (int j = threadIdx.x; j < nt * A; j += kRotThreads) {
@@ -174,27 +191,23 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(RotaryArgs a, Ro
     for (; i < work; i += kRotThreads) {
         if (i >= kRotThreads) {
             place(i);
-            fetch(hg);
+            fetch();
         }
         Turn<T, VP, IL> tn;
         if (turn) tn.load(cs + tl * P + slot * VP);
-        const int64_t t = t0 + tl;
-        T* qo = static_cast<T*>(a.q_out) + t * a.Hq * a.D;
-        T* ko = static_cast<T*>(a.k_out) + t * a.Hk * a.D;
-        for (int h0 = hg;;) {
+        for (;;) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h = h0 + u * pl.hgroups;
-                if (h < H) {
-                    T* dst = h < Hq ? qo + int64_t(h) * a.D : ko + int64_t(h - Hq) * a.D;
+            for (int u = 0; u < U; ++u)
+                if (u < heads) {
                     if (turn) tn(p0[u], p1[u]);
-                    store_pack<T, VP>(dst + o0, p0[u]);
-                    if (second) store_pack<T, VP>(dst + o1, p1[u]);
+                    store_pack<T, VP>(dst + u * a.D, p0[u]);
+                    if (second) store_pack<T, VP>(dst + u * a.D + o1, p1[u]);
                 }
-            }
-            h0 += U * pl.hgroups;
-            if (h0 >= H) break;
-            fetch(h0);
+            heads -= U;
+            if (heads <= 0) break;
+            src += U * stride;
+            dst += U * a.D;
+            fetch();
         }
     }
 }
@@ -206,11 +219,12 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
     pl.pair_slots = int(a.P / VP);
     pl.slots = pl.pair_slots + int(ceil_div(ceil_div(a.D - 2 * a.P, VP), 2));
     const int64_t H = a.Hq + a.Hk;
-    // Heads side by side: all of them for a few tokens (one access each, so a
-    // small call is one round trip); four to a thread, loaded together, where
-    // that alone fills the GPU.
-    pl.hgroups = int(pl.ntok * pl.slots * H <= int64_t(148) * 2048 ? H : ceil_div(H, 4));
-    const int64_t per_token = int64_t(pl.slots) * pl.hgroups;
+    // A head a thread for a few tokens (one access each, so a small call is one
+    // round trip), runs of heads where those alone fill the GPU.
+    pl.run = pl.ntok * pl.slots * H <= int64_t(148) * 2048 ? 1 : kRotRun;
+    pl.q_runs = int(ceil_div(a.Hq, pl.run));
+    pl.runs = pl.q_runs + int(ceil_div(a.Hk, pl.run));
+    const int64_t per_token = int64_t(pl.slots) * pl.runs;
     int64_t tokens = per_token >= kRotThreads ? 1 : kRotThreads / per_token;
     const int64_t fit = a.P > 0 ? kMaxPairs / a.P : tokens;
     if (tokens > fit) tokens = fit;

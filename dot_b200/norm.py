@@ -33,32 +33,43 @@ class _GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, lengths, num_groups: int, eps: float, activation: int):
         y, stats = ops.group_norm_forward_raw(x, num_groups, weight, bias, eps, activation, lengths)
         ctx.save_for_backward(x, weight, bias, lengths, stats)
-        ctx.num_groups = num_groups
-        ctx.activation = activation
+        ctx.groups_act = (num_groups, activation)
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
+    def _grads(ctx, dy):
         x, weight, bias, lengths, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = ops.group_norm_backward_raw(x, dy, ctx.num_groups, weight, bias, ctx.activation, stats, lengths,
-                                                 need[0], need[1], need[2])
+        num_groups, activation = ctx.groups_act
+        dx, dw, db = ops.group_norm_backward_raw(x, dy, num_groups, weight, bias, activation, stats, lengths,
+                                                 *ctx.needs_input_grad[:3])
         return dx, dw, db, None, None, None, None
+
+    _grads_once = staticmethod(once_differentiable(_grads.__func__))
+
+    @staticmethod
+    def backward(ctx, dy):
+        # the wrapper that refuses a second differentiation is needed where one is recorded
+        if torch.is_grad_enabled():
+            return _GroupNormActFn._grads_once(ctx, dy)
+        return _GroupNormActFn._grads(ctx, dy)
+
+
+_ACTIVATION_CODES = {name: code for code, name in enumerate(_lib.ACTIVATIONS)}
 
 
 def _activation_code(activation: str) -> int:
-    try:
-        return _lib.ACTIVATIONS.index(activation)
-    except ValueError:
-        raise ValueError(f"activation must be one of {', '.join(_lib.ACTIVATIONS)}, got {activation!r}") from None
+    code = _ACTIVATION_CODES.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be one of {', '.join(_lib.ACTIVATIONS)}, got {activation!r}")
+    return code
 
 
-def _check_param(p: torch.Tensor, C: int, name: str, dev: torch.device) -> None:
+def _check_param(p: torch.Tensor, C: int, name: str, x: torch.Tensor) -> torch.Tensor:
     if p.dim() != 1 or p.size(0) != C:
         raise ValueError(f"{name} must have shape [{C}]")
-    if p.device != dev:
-        raise ValueError(f"{name} must be on {dev}")
+    if p.get_device() != x.get_device():
+        raise ValueError(f"{name} must be on {x.device}")
+    return p if p.is_contiguous() else p.contiguous()
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -83,26 +94,27 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     if not eps >= 0:
         raise ValueError("eps must be >= 0")
     act = _activation_code(activation)
+    grad = x.requires_grad
     if weight is not None:
-        _check_param(weight, C, "weight", x.device)
+        weight = _check_param(weight, C, "weight", x)
+        grad = grad or weight.requires_grad
     if bias is not None:
-        _check_param(bias, C, "bias", x.device)
-    both = [p for p in (weight, bias) if p is not None]
-    if any(p.dtype not in ops._FEATURE_DTYPES or p.dtype != both[0].dtype for p in both):
-        weight, bias = (None if p is None else p.to(torch.float32) for p in (weight, bias))
-    if weight is not None:
-        weight = weight.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
+        bias = _check_param(bias, C, "bias", x)
+        grad = grad or bias.requires_grad
+    dt = x.dtype if weight is None else weight.dtype
+    if dt not in ops._FEATURE_DTYPES or (bias is not None and bias.dtype != dt):
+        # the kernels read both parameters as one type
+        weight = None if weight is None else weight.to(torch.float32)
+        bias = None if bias is None else bias.to(torch.float32)
     if lengths is not None:
         if lengths.dim() != 1 or lengths.size(0) != x.size(0):
             raise ValueError("lengths must be [N]")
         if lengths.dtype != torch.int32:
             raise ValueError("lengths must be int32")
         lengths = lengths.to(x.device).contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in both)):
-        return _GroupNormActFn.apply(x, weight, bias, lengths, int(num_groups), float(eps), act)
-    return ops.group_norm_forward_raw(x, int(num_groups), weight, bias, float(eps), act, lengths)[0]
+    if grad and torch.is_grad_enabled():
+        return _GroupNormActFn.apply(x, weight, bias, lengths, num_groups, eps, act)
+    return ops.group_norm_forward_raw(x, num_groups, weight, bias, eps, act, lengths)[0]
 
 
 class GroupNormAct(nn.Module):

@@ -21,7 +21,6 @@ from __future__ import annotations
 
 import functools
 import math
-from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -227,9 +226,22 @@ _FEATURE_DTYPES = {torch.float32: _lib.DOT_F32, torch.bfloat16: _lib.DOT_BF16, t
 _POSITION_DTYPES = {torch.int32: _lib.DOT_I32, torch.int64: _lib.DOT_I64, torch.float32: _lib.DOT_F32}
 
 
-def _on(t: torch.Tensor):
-    """Makes ``t``'s device current for a launch, where it is not."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+class _Current:
+    """Makes a device current for a launch, where it is not."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def _rows(x: torch.Tensor):
@@ -258,30 +270,36 @@ def _rows(x: torch.Tensor):
 
 
 @functools.lru_cache(maxsize=1024)
-def _norm_workspace_bytes(N: int, S: int, C: int, G: int, backward: bool) -> int:
+def _norm_scratch(N: int, S: int, C: int, G: int, backward: bool):
+    """Workspace bytes of a group norm call and, for the forward, the floats of the one buffer that holds
+    the statistics (first) and the workspace, with the workspace's offset in bytes."""
     lib = _lib.load()
-    return (lib.dot_group_norm_bwd_workspace_bytes if backward else lib.dot_group_norm_fwd_workspace_bytes)(N, S, C, G)
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    if backward:
+        nbytes = lib.dot_group_norm_bwd_workspace_bytes(N, S, C, G)
+        return nbytes, nbytes, 0
+    nbytes = lib.dot_group_norm_fwd_workspace_bytes(N, S, C, G)
+    at = -(-(N * G * 8) // 256) * 256
+    return nbytes, (at + nbytes) // 4, at
 
 
 def group_norm_forward_raw(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor],
                            bias: Optional[torch.Tensor], eps: float, activation: int,
                            lengths: Optional[torch.Tensor] = None):
-    """One call of ``dot_group_norm_fwd`` on x [N, *S, C]; returns ``(y, stats [N,G,2])``."""
+    """One call of ``dot_group_norm_fwd`` on x [N, *S, C]; returns ``(y, stats)``: stats is a flat float32
+    buffer that begins with the [N,G,2] statistics (scratch space follows)."""
     x, N, S, C, xb, xp = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((N, num_groups, 2), dtype=torch.float32, device=x.device)
-    nbytes = _norm_workspace_bytes(N, S, C, num_groups, False)
-    ws = _lib.workspace(nbytes, x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    nbytes, nfloats, at = _norm_scratch(N, S, C, num_groups, False)
+    stats = x.new_empty((nfloats,), dtype=torch.float32)
     p = weight if weight is not None else bias
-    with _on(x):
+    dev = x.get_device()
+    with _Current(dev):
+        sp = stats.data_ptr()
         rc = _lib.load().dot_group_norm_fwd(
-            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, _ptr(weight), _ptr(bias),
-            _lib.DOT_F32 if p is None else _FEATURE_DTYPES[p.dtype], _ptr(lengths), N, S, C, num_groups, eps,
-            activation, y.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes, _lib.stream_of(x))
+            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), 0 if p is None else _FEATURE_DTYPES[p.dtype],
+            None if lengths is None else lengths.data_ptr(), N, S, C, num_groups, eps, activation, y.data_ptr(), sp,
+            sp + at, nbytes, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "dot_group_norm_fwd")
     return y, stats
@@ -291,33 +309,31 @@ def group_norm_backward_raw(x: torch.Tensor, dy: torch.Tensor, num_groups: int, 
                             bias: Optional[torch.Tensor], activation: int, stats: torch.Tensor,
                             lengths: Optional[torch.Tensor] = None, want_dx: bool = True,
                             want_dweight: bool = True, want_dbias: bool = True):
-    """One call of ``dot_group_norm_bwd``; returns ``(dx, dweight, dbias)``, None where not wanted."""
+    """One call of ``dot_group_norm_bwd``; returns ``(dx, dweight, dbias)``, None where not wanted (or
+    where there is no such parameter)."""
     x, N, S, C, xb, xp = _rows(x)
     dy, _, _, _, gb, gp = _rows(dy)
     p = weight if weight is not None else bias
-    pdt = torch.float32 if p is None else p.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty((C,), dtype=pdt, device=x.device) if want_dweight else None
-    db = torch.empty((C,), dtype=pdt, device=x.device) if want_dbias else None
-    nbytes = _norm_workspace_bytes(N, S, C, num_groups, True)
-    ws = _lib.workspace(nbytes, x.device)
-    with _on(x):
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
+    dw = torch.empty_like(weight) if want_dweight and weight is not None else None
+    db = torch.empty_like(bias) if want_dbias and bias is not None else None
+    nbytes = _norm_scratch(N, S, C, num_groups, True)[0]
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    dev = x.get_device()
+    with _Current(dev):
         rc = _lib.load().dot_group_norm_bwd(
-            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, dy.data_ptr(), gb, gp, _ptr(weight), _ptr(bias),
-            _FEATURE_DTYPES[pdt], _ptr(lengths), N, S, C, num_groups, activation, stats.data_ptr(), _ptr(dx),
-            _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_of(x))
+            x.data_ptr(), _FEATURE_DTYPES[x.dtype], xb, xp, dy.data_ptr(), gb, gp,
+            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+            0 if p is None else _FEATURE_DTYPES[p.dtype], None if lengths is None else lengths.data_ptr(), N, S, C,
+            num_groups, activation, stats.data_ptr(), None if dx is None else dx.data_ptr(),
+            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), nbytes,
+            _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "dot_group_norm_bwd")
     return dx, dw, db
 
 
-def _heads(x: torch.Tensor) -> torch.Tensor:
-    """``x`` with consecutive elements within a head."""
-    return x if x.stride(-1) == 1 or x.size(-1) == 1 else x.contiguous()
-
-
-def _i64x3(a: int, b: int, c: int):
-    return (_lib.ctypes.c_int64 * 3)(a, b, c)
+_I64x3 = _lib.ctypes.c_int64 * 3
 
 
 def rotary_raw(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor,
@@ -326,26 +342,35 @@ def rotary_raw(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: 
     freqs [P,A]; returns ``(q', k')``, None where the input is None."""
     ref = q if q is not None else k
     B, L, _, D = ref.shape
-    outs, args = [], []
-    for t in (q, k):
-        if t is None:
-            outs.append(None)
-            args.append((None, None, 0))
-            continue
-        t = _heads(t)
-        outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
-        args.append((t, _i64x3(t.stride(0), t.stride(1), t.stride(2)), t.size(2)))
-    (q, qs, hq), (k, ks, hk) = args
+    qs = ks = qp = kp = qop = kop = qo = ko = None
+    hq = hk = 0
+    if q is not None:
+        s = q.stride()
+        if s[3] != 1 and D != 1:    # elements of a head are consecutive
+            q = q.contiguous()
+            s = q.stride()
+        hq = q.size(2)
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        qs, qp, qop = _I64x3(s[0], s[1], s[2]), q.data_ptr(), qo.data_ptr()
+    if k is not None:
+        s = k.stride()
+        if s[3] != 1 and D != 1:
+            k = k.contiguous()
+            s = k.stride()
+        hk = k.size(2)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ks, kp, kop = _I64x3(s[0], s[1], s[2]), k.data_ptr(), ko.data_ptr()
     P, A = freqs.shape
-    ps = _i64x3(positions.stride(0) if positions.size(0) == B else 0, positions.stride(1), positions.stride(2))
-    with _on(ref):
+    s = positions.stride()
+    dev = ref.get_device()
+    with _Current(dev):
         rc = _lib.load().dot_rotary(
-            _ptr(q), qs, hq, _ptr(k), ks, hk, _FEATURE_DTYPES[ref.dtype], positions.data_ptr(),
-            _POSITION_DTYPES[positions.dtype], ps, freqs.data_ptr(), B, L, D, P, A, 1 if interleaved else 0,
-            1 if inverse else 0, _ptr(outs[0]), _ptr(outs[1]), _lib.stream_of(ref))
+            qp, qs, hq, kp, ks, hk, _FEATURE_DTYPES[ref.dtype], positions.data_ptr(),
+            _POSITION_DTYPES[positions.dtype], _I64x3(s[0] if positions.size(0) == B else 0, s[1], s[2]),
+            freqs.data_ptr(), B, L, D, P, A, interleaved, inverse, qop, kop, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "dot_rotary")
-    return outs[0], outs[1]
+    return qo, ko
 
 
 # ---- reference-named ops ------------------------------------------------------

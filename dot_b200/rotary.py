@@ -36,14 +36,15 @@ class _RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
+        need = ctx.needs_input_grad
+        if not need[0]:
+            dq = None
+        if not need[1]:
+            dk = None
         if dq is None and dk is None:
             return (None,) * 6
         positions, freqs = ctx.saved_tensors
         interleaved, inverse = ctx.flags
-        if not ctx.needs_input_grad[0]:
-            dq = None
-        if not ctx.needs_input_grad[1]:
-            dk = None
         # the turn is orthogonal: its backward is the turn by -angle
         turn = _RotaryFn.apply if torch.is_grad_enabled() else ops.rotary_raw
         dq, dk = turn(dq, dk, positions, freqs, interleaved, not inverse)
@@ -60,8 +61,6 @@ def _check_heads(x: torch.Tensor, name: str) -> None:
 
 
 def _as_4d(x: torch.Tensor) -> torch.Tensor:
-    if x.dim() == 4:
-        return x
     if x.dim() == 3:
         return x.unsqueeze(0)
     return x.reshape(math.prod(x.shape[:-3]), *x.shape[-3:])
@@ -79,40 +78,44 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Opt
     k is given.  Differentiable in q and k, not in positions or freqs.
     """
     _check_heads(q, "q")
+    shape = q.shape
+    lead = shape[:-2]
+    grad = q.requires_grad
     if k is not None:
         _check_heads(k, "k")
-        if k.shape[:-2] != q.shape[:-2] or k.size(-1) != q.size(-1):
+        if k.shape[:-2] != lead or k.size(-1) != shape[-1]:
             raise ValueError("k must have q's shape except for the number of heads")
-        if k.dtype != q.dtype or k.device != q.device:
+        if k.dtype != q.dtype or k.get_device() != q.get_device():
             raise ValueError("k must have q's dtype and device")
+        grad = grad or k.requires_grad
     if freqs.dim() != 2 or freqs.dtype != torch.float32:
         raise ValueError("freqs must be float32 [P, A]")
     if positions.dtype not in ops._POSITION_DTYPES:
         raise ValueError("positions must be int32, int64 or float32")
-    if positions.device != q.device or freqs.device != q.device:
+    if positions.get_device() != q.get_device() or freqs.get_device() != q.get_device():
         raise ValueError("positions and freqs must be on q's device")
     if positions.requires_grad or freqs.requires_grad:
         raise ValueError("positions and freqs are not differentiable here: detach them")
     P, A = freqs.shape
     if not 1 <= A <= 4:
         raise ValueError("freqs must have 1 to 4 axes")
-    if 2 * P > q.size(-1):
+    if 2 * P > shape[-1]:
         raise ValueError("freqs must hold at most D/2 pairs")
-    L = q.size(-3)
-    if positions.shape != (*q.shape[:-2], A):
-        if positions.shape != (L, A):
+    if positions.shape != (*lead, A):
+        if positions.shape != (lead[-1], A):
             raise ValueError("positions must be [*, L, A] with q's leading axes, or [L, A]")
         positions = positions.unsqueeze(0)
-    elif positions.dim() != 3:
-        positions = positions.reshape(math.prod(q.shape[:-3]), L, A)
-    q4, k4 = _as_4d(q), None if k is None else _as_4d(k)
-    freqs = freqs.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    elif len(lead) != 2:
+        positions = positions.reshape(math.prod(lead[:-1]), lead[-1], A)
+    if not freqs.is_contiguous():
+        freqs = freqs.contiguous()
+    q4, k4 = (q, k) if len(lead) == 2 else (_as_4d(q), None if k is None else _as_4d(k))
+    if grad and torch.is_grad_enabled():
         q4, k4 = _RotaryFn.apply(q4, k4, positions, freqs, bool(interleaved), False)
     else:
         q4, k4 = ops.rotary_raw(q4, k4, positions, freqs, bool(interleaved))
-    if q.dim() != 4:
-        q4 = q4.view(q.shape)
+    if len(lead) != 2:
+        q4 = q4.view(shape)
         k4 = None if k is None else k4.view(k.shape)
     return q4 if k is None else (q4, k4)
 
