@@ -194,8 +194,8 @@ template <int ACT>
 __device__ __forceinline__ float2 act_slope(float2 z, int act_rt) {
     const int act = ACT >= 0 ? ACT : act_rt;
     if (act == kActSilu) {
-        const float2 s = sigmoid2(z);   // s + z s (1 - s)
-        return fma2(z, fma2(mul2(s, splat2(-1.0f)), s, s), s);
+        const float2 s = sigmoid2(z);
+        return fma2(z, sub2(s, mul2(s, s)), s);   // s + z s (1 - s)
     }
     if (act == kActGelu) {
         const float2 pdf = mul2(ex2_2(mul2(mul2(z, splat2(-0.5f * kLog2e)), z)), splat2(0.39894228f));

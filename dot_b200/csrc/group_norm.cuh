@@ -48,7 +48,6 @@ constexpr int res_vecs(int bytes, bool backward) {
 
 struct GnPlan {
     GroupNormArgs a;
-    int n0;              // sweeps: first sample of this launch
     int chunks;          // blocks that share a sample's positions
     int rows;            // positions per chunk
     int slab_groups;     // resident: groups of a block's channel slab
@@ -155,36 +154,29 @@ struct PerGroup {
     }
 };
 
-// y of a vector.  16-bit values take the mean with the shift (one fma); float32
-// subtracts it first, since the rounding of a large mean * scale would show.
+// y of a vector.  The mean is subtracted first rather than taken into the shift:
+// a group of equal values then gives its bias exactly.
 template <typename T, int VEC, int ACT, bool ONEG>
 struct Forward {
     static constexpr int NP = pairs_of(VEC);
-    static constexpr bool FOLD = sizeof(T) == 2;
-    PerGroup<VEC, ONEG || FOLD> mean;   // unused where folded
+    PerGroup<VEC, ONEG> mean;
     float2 scale[NP], shift[NP];
     // st: (mean, rstd) by group; c: the first channel, c_st: counted from st's first group
     __device__ __forceinline__ void load(const GroupNormArgs& a, int c, int c_st, int Cg, const float2* st) {
         load_params<VEC>(a.weight, a.param_dtype, c, 1.0f, scale);
         load_params<VEC>(a.bias, a.param_dtype, c, 0.0f, shift);
-        PerGroup<VEC, ONEG> m, r;
-        m.fill(c_st, Cg, [&](int g) { return st[g].x; });
+        mean.fill(c_st, Cg, [&](int g) { return st[g].x; });
+        PerGroup<VEC, ONEG> r;
         r.fill(c_st, Cg, [&](int g) { return st[g].y; });
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            scale[j] = mul2(scale[j], r[j]);
-            if constexpr (FOLD)
-                shift[j] = fma2(make_float2(-m[j].x, -m[j].y), scale[j], shift[j]);
-            else
-                mean.v[ONEG ? 0 : j] = m[j];
-        }
+        for (int j = 0; j < NP; ++j) scale[j] = mul2(scale[j], r[j]);
     }
     __device__ __forceinline__ Pack<T, VEC> operator()(const Pack<T, VEC>& raw, int act) const {
         float2 f[NP];
         unpack(raw, f);
 #pragma unroll
         for (int j = 0; j < NP; ++j)
-            f[j] = act_fwd<ACT>(fma2(FOLD ? f[j] : sub2(f[j], mean[j]), scale[j], shift[j]), act);
+            f[j] = act_fwd<ACT>(fma2(sub2(f[j], mean[j]), scale[j], shift[j]), act);
         return pack<T, VEC>(f);
     }
 };
@@ -220,21 +212,39 @@ struct Backward {
             sb[j] = fma2(dz, xh, sb[j]);
         }
     }
-    // s1, s2: the group's S1/m and S2/m
-    __device__ __forceinline__ Pack<T, VEC> dx(const Pack<T, VEC>& rx, const Pack<T, VEC>& rg, int act,
-                                               const PerGroup<VEC, ONEG>& s1, const PerGroup<VEC, ONEG>& s2) const {
+};
+
+// dx = (rstd w) dz - rstd S1/m - xh (rstd S2/m)
+template <typename T, int VEC, int ACT, bool ONEG>
+struct BackwardDx : Backward<T, VEC, ACT, ONEG> {
+    using Base = Backward<T, VEC, ACT, ONEG>;
+    static constexpr int NP = Base::NP;
+    PerGroup<VEC, ONEG> s1, s2;   // -rstd S1/m, -rstd S2/m
+    float2 rw[NP];
+    // sum(g): group g's (S1/m, S2/m).  A group of one value has no gradient.
+    template <typename F>
+    __device__ __forceinline__ void finish(int c_st, int Cg, int len, F sum) {
+        const float on = int64_t(len) * Cg > 1 ? 1.0f : 0.0f;
+        s1.fill(c_st, Cg, [&](int g) { return -on * sum(g).x; });
+        s2.fill(c_st, Cg, [&](int g) { return -on * sum(g).y; });
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            rw[j] = mul2(mul2(this->rstd[j], splat2(on)), this->w[j]);
+            if (!ONEG || j == 0) {
+                s1.v[j] = mul2(s1.v[j], this->rstd[j]);
+                s2.v[j] = mul2(s2.v[j], this->rstd[j]);
+            }
+        }
+    }
+    __device__ __forceinline__ Pack<T, VEC> dx(const Pack<T, VEC>& rx, const Pack<T, VEC>& rg, int act) const {
         float2 x[NP], g[NP];
         unpack(rx, x);
         unpack(rg, g);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             float2 xh, dz;
-            chain(x[j], g[j], j, act, xh, dz);
-            // w dz rounded as in its sum (a scalar product is not contracted): the
-            // gradient of a group of one value is 0
-            const float2 wdz = make_float2(__fmul_rn(w[j].x, dz.x), __fmul_rn(w[j].y, dz.y));
-            const float2 t = sub2(wdz, s1[j]), n = mul2(xh, splat2(-1.0f));
-            x[j] = mul2(rstd[j], fma2(n, s2[j], t));
+            this->chain(x[j], g[j], j, act, xh, dz);
+            x[j] = fma2(xh, s2[j], fma2(rw[j], dz, s1[j]));
         }
         return pack<T, VEC>(x);
     }
@@ -368,7 +378,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G] mean, M of the tiles so far
     float2* part = acc + G;                             // [rp][nv * W]
-    const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
         if (pc.on) {
             PerGroup<VEC, ONEG> pivot;
             pivot.fill(c0 + pc.v * VEC, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
-            const T* xc = x + c0 + pc.v * VEC;
+            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c0 + pc.v * VEC;
             const int64_t step = int64_t(pc.rp) * a.xp;
             float n_run = 0.0f, mean[W], m2[W];
 #pragma unroll
@@ -395,24 +405,21 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
                 }
                 n_run = tot;
             };
-            int p = p0 + pc.r;
-            for (; p + (U - 1) * pc.rp < p1; p += U * pc.rp) {
+            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+            for (; left >= U; left -= U) {
                 Pack<T, VEC> raw[U];
-                const T* at = xc + int64_t(p) * a.xp;
 #pragma unroll
-                for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * step);
+                for (int u = 0; u < U; ++u, xc += step) raw[u] = load_pack<T, VEC>(xc);
                 bt.template take<U, true>(raw, pivot, U);
                 join(float(U));
             }
-            if (p < p1) {
+            if (left > 0) {
                 Pack<T, VEC> raw[U];
-                const T* at = xc + int64_t(p) * a.xp;
-                const int k = (p1 - p + pc.rp - 1) / pc.rp;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (u < k) raw[u] = load_pack<T, VEC>(at + u * step);
-                bt.template take<U, false>(raw, pivot, k);
-                join(float(k));
+                for (int u = 0; u < U; ++u, xc += step)
+                    if (u < left) raw[u] = load_pack<T, VEC>(xc);
+                bt.template take<U, false>(raw, pivot, left);
+                join(float(left));
             }
 #pragma unroll
             for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(mean[j], m2[j]);
@@ -445,7 +452,6 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
         }
         __syncthreads();
     }
-    pdl_wait();   // the launches before this one are done when it is
     for (int g = threadIdx.x; g < G; g += kGnThreads)
         pl.moments[(int64_t(n) * pl.chunks + chunk) * G + g] = acc[g];
 }
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
     float2* st = reinterpret_cast<float2*>(gn_smem);   // [G] mean, rstd
     constexpr int U = 8;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
@@ -499,20 +505,20 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
         const int c = (tile * kGnThreads + pc.v) * VEC;
         Forward<T, VEC, ACT, ONEG> fw;
         fw.load(a, c, c, Cg, st);
-        auto write = [&](int p, const Pack<T, VEC>& raw) {
-            store_pack<T, VEC>(y + int64_t(p) * C + c, fw(raw, a.act));
-        };
         for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
             store_pack<T, VEC>(y + int64_t(p) * C + c, pack_zero<T, VEC>());
-        int p = pv - 1 - pc.r;
-        for (; p - (U - 1) * pc.rp >= p0; p -= U * pc.rp) {
+        int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
+        const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
+        T* yc = y + int64_t(pv - 1 - pc.r) * C + c;
+        const int64_t xs = int64_t(pc.rp) * a.xp, ys = int64_t(pc.rp) * C;
+        for (; left >= U; left -= U) {
             Pack<T, VEC> raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(x + int64_t(p - u * pc.rp) * a.xp + c);
+            for (int u = 0; u < U; ++u, xc -= xs) raw[u] = load_pack<T, VEC>(xc);
 #pragma unroll
-            for (int u = 0; u < U; ++u) write(p - u * pc.rp, raw[u]);
+            for (int u = 0; u < U; ++u, yc -= ys) store_pack<T, VEC>(yc, fw(raw[u], a.act));
         }
-        for (; p >= p0; p -= pc.rp) write(p, load_pack<T, VEC>(x + int64_t(p) * a.xp + c));
+        for (; left > 0; --left, xc -= xs, yc -= ys) store_pack<T, VEC>(yc, fw(load_pack<T, VEC>(xc), a.act));
     }
 }
 
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G]
     float2* part = acc + G;                             // [rp][nv * VEC]
-    const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int64_t slot = int64_t(n) * pl.chunks + chunk;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
@@ -546,20 +552,22 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
             float2 sa[NP], sb[NP];
 #pragma unroll
             for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
-            auto take = [&](const Pack<T, VEC>& rx, const Pack<T, VEC>& rg) { bw.sums(rx, rg, a.act, sa, sb); };
-            int p = p0 + pc.r;
-            for (; p + (U - 1) * pc.rp < p1; p += U * pc.rp) {
+            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
+            const T* gc = dy + int64_t(p0 + pc.r) * a.gp + c;
+            const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp;
+            for (; left >= U; left -= U) {
                 Pack<T, VEC> rx[U], rg[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    rx[u] = load_pack<T, VEC>(x + int64_t(p + u * pc.rp) * a.xp + c);
-                    rg[u] = load_pack<T, VEC>(dy + int64_t(p + u * pc.rp) * a.gp + c);
+                for (int u = 0; u < U; ++u, xc += xs, gc += gs) {
+                    rx[u] = load_pack<T, VEC>(xc);
+                    rg[u] = load_pack<T, VEC>(gc);
                 }
 #pragma unroll
-                for (int u = 0; u < U; ++u) take(rx[u], rg[u]);
+                for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
             }
-            for (; p < p1; p += pc.rp)
-                take(load_pack<T, VEC>(x + int64_t(p) * a.xp + c), load_pack<T, VEC>(dy + int64_t(p) * a.gp + c));
+            for (; left > 0; --left, xc += xs, gc += gs)
+                bw.sums(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act, sa, sb);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
                 part[(pc.r * pc.nv + pc.v) * VEC + j] =
@@ -598,7 +606,6 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
         }
         __syncthreads();
     }
-    pdl_wait();   // the launches before this one are done when it is
     for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
 }
 
@@ -610,7 +617,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     float4* gv = reinterpret_cast<float4*>(gn_smem);   // [G] mean, rstd, S1/m, S2/m
     constexpr int U = 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    const int n = pl.n0 + int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv = len > 0 ? 1.0f / (float(len) * float(Cg)) : 0.0f;
@@ -650,29 +657,28 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
         const Place pc(cv, tile);
         if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
-        Backward<T, VEC, ACT, ONEG> bw;
+        BackwardDx<T, VEC, ACT, ONEG> bw;
         bw.load(a, c, c, Cg, gv);
-        PerGroup<VEC, ONEG> s1, s2;
-        s1.fill(c, Cg, [&](int g) { return gv[g].z; });
-        s2.fill(c, Cg, [&](int g) { return gv[g].w; });
-        auto write = [&](int p, const Pack<T, VEC>& rx, const Pack<T, VEC>& rg) {
-            store_pack<T, VEC>(dx + int64_t(p) * C + c, bw.dx(rx, rg, a.act, s1, s2));
-        };
+        bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
         for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
             store_pack<T, VEC>(dx + int64_t(p) * C + c, pack_zero<T, VEC>());
-        int p = pv - 1 - pc.r;
-        for (; p - (U - 1) * pc.rp >= p0; p -= U * pc.rp) {
+        int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
+        const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
+        const T* gc = dy + int64_t(pv - 1 - pc.r) * a.gp + c;
+        T* dc = dx + int64_t(pv - 1 - pc.r) * C + c;
+        const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp, ds = int64_t(pc.rp) * C;
+        for (; left >= U; left -= U) {
             Pack<T, VEC> rx[U], rg[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                rx[u] = load_pack<T, VEC>(x + int64_t(p - u * pc.rp) * a.xp + c);
-                rg[u] = load_pack<T, VEC>(dy + int64_t(p - u * pc.rp) * a.gp + c);
+            for (int u = 0; u < U; ++u, xc -= xs, gc -= gs) {
+                rx[u] = load_pack<T, VEC>(xc);
+                rg[u] = load_pack<T, VEC>(gc);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) write(p - u * pc.rp, rx[u], rg[u]);
+            for (int u = 0; u < U; ++u, dc -= ds) store_pack<T, VEC>(dc, bw.dx(rx[u], rg[u], a.act));
         }
-        for (; p >= p0; p -= pc.rp)
-            write(p, load_pack<T, VEC>(x + int64_t(p) * a.xp + c), load_pack<T, VEC>(dy + int64_t(p) * a.gp + c));
+        for (; left > 0; --left, xc -= xs, gc -= gs, dc -= ds)
+            store_pack<T, VEC>(dc, bw.dx(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act));
     }
 }
 
@@ -814,7 +820,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan p
         }
     }
     const float2* stats = reinterpret_cast<const float2*>(a.stats) + int64_t(pc.n) * G + pc.g0;
-    Backward<T, VEC, ACT, ONEG> bw;
+    BackwardDx<T, VEC, ACT, ONEG> bw;
     if (pc.on) {
         bw.load(a, c, pc.v * VEC, Cg, stats);
         constexpr int NP = pairs_of(VEC);
@@ -880,15 +886,13 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan p
     __syncthreads();
     if (pc.on && a.dx != nullptr) {
         T* dx = static_cast<T*>(a.dx) + int64_t(pc.n) * a.S * C + c;
-        PerGroup<VEC, ONEG> s1, s2;
-        s1.fill(pc.v * VEC, Cg, [&](int g) { return sums[g].x; });
-        s2.fill(pc.v * VEC, Cg, [&](int g) { return sums[g].y; });
+        bw.finish(pc.v * VEC, Cg, len, [&](int g) { return sums[g]; });
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int p = p0 + pc.r + k * pc.rp;
             if (p >= pe) break;
             store_pack<T, VEC>(dx + int64_t(p) * C,
-                               k < cnt ? bw.dx(rx[k], rg[k], a.act, s1, s2) : pack_zero<T, VEC>());
+                               k < cnt ? bw.dx(rx[k], rg[k], a.act) : pack_zero<T, VEC>());
         }
     }
     if (pl.chunks > 1) cl_wait();     // no block leaves while a peer may read its sums
@@ -896,20 +900,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan p
 
 // ---- host ---------------------------------------------------------------------
 
-// Sweeps: samples are taken in batches whose x (and dy) the L2 cache still
-// holds when the second sweep reads them again.
-constexpr int64_t kBatchBytes = int64_t(48) << 20;
-
-void sweep_plan(GnPlan& pl, int esz, bool backward, int& batch) {
+// Sweeps: one block per SM over all samples, at least 32 positions each.
+void sweep_plan(GnPlan& pl) {
     const GroupNormArgs& a = pl.a;
-    const int64_t bytes = a.S * a.C * esz * (backward ? 2 : 1);
-    int64_t nb = kBatchBytes / (bytes > 0 ? bytes : 1);
-    nb = nb < 1 ? 1 : nb > a.N ? a.N : nb;
-    nb = ceil_div(a.N, ceil_div(a.N, nb));   // batches of one size
-    // one block per SM over a batch, at least 32 positions each
-    int64_t want = kSMs / nb < 1 ? 1 : kSMs / nb;
+    int64_t want = kSMs / a.N < 1 ? 1 : kSMs / a.N;
     if (want > ceil_div(a.S, 32)) want = ceil_div(a.S, 32);
-    batch = int(nb);
     pl.rows = int(ceil_div(a.S, want));
     pl.chunks = int(ceil_div(a.S, pl.rows));
 }
@@ -934,16 +929,11 @@ size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward
     pl.a.S = S;
     pl.a.C = C;
     pl.a.G = G;
-    size_t most = 0;
-    for (int esz = 2; esz <= 4; esz += 2) {
-        int batch;
-        sweep_plan(pl, esz, backward, batch);
-        const size_t b = carve(nullptr, pl, backward);
-        if (b > most) most = b;
-    }
-    pl.chunks = kMaxCluster;   // resident
-    const size_t b = backward ? carve(nullptr, pl, true) : 0;
-    return b > most ? b : most;
+    sweep_plan(pl);
+    const size_t sweeps = carve(nullptr, pl, backward);
+    pl.chunks = kMaxCluster;   // resident: needs none forward
+    const size_t resident = backward ? carve(nullptr, pl, true) : 0;
+    return sweeps > resident ? sweeps : resident;
 }
 
 template <typename K>
@@ -1037,25 +1027,23 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
 template <typename T, int VEC, int ACT, bool ONEG>
 int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     const GroupNormArgs& a = pl.a;
-    int batch;
-    sweep_plan(pl, sizeof(T), backward, batch);
+    sweep_plan(pl);
     carve(ws, pl, backward);
     const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
     const size_t s1 = (size_t(a.G) + part) * sizeof(float2);
     const size_t s2 = size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
-    for (int64_t n = 0; n < a.N; n += batch) {
-        pl.n0 = int(n);
-        const int64_t blocks = (a.N - n < batch ? a.N - n : batch) * pl.chunks;
-        const bool second = !backward || a.dx != nullptr;
+    const int64_t blocks = a.N * pl.chunks;
+    const bool second = !backward || a.dx != nullptr;
+    int rc;
+    {
         ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st, second ? 2 : 1);
-        int rc = backward
-            ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, n > 0, st)
-            : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, n > 0, st);
+        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, false, st)
+                      : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, false, st);
         if (!rc && second)
             rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st)
                           : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st);
-        if (rc) return rc;
     }
+    if (rc) return rc;
     return backward ? launch_params(pl, st) : DOT_OK;
 }
 
