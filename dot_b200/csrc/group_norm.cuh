@@ -301,6 +301,86 @@ struct Place {
     }
 };
 
+// A ring of bulk copies for rows that lie one after another in memory: 192 KB
+// in flight per SM without a register.  A stage holds U rows for each row
+// position of the block, of x and for NT = 2 of dy; the last of the 16 warps to
+// leave a stage refills it.  Waits are bounded: one that expires makes the
+// block go on without waiting, and its results are written as NaN.
+constexpr int kRingStages = 6;
+constexpr int kRingStageBytes = 32 * 1024;
+
+template <int NT>
+struct Ring {
+    static constexpr int kPart = kRingStageBytes / NT;   // bytes of one tensor in a stage
+    unsigned char* buf;
+    uint64_t* full;                     // [kRingStages]
+    int* left;                          // [kRingStages] warps that have left the stage
+    const unsigned char* src[NT];       // row 0 of the block's range
+    int row_bytes, rows, stage_rows, n; // rows in all, per stage; stages
+    bool reverse, dead = false;
+
+    static constexpr size_t bytes() { return size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + sizeof(int)); }
+    __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_, bool reverse_) {
+        buf = smem;
+        full = reinterpret_cast<uint64_t*>(smem + kRingStages * kRingStageBytes);
+        left = reinterpret_cast<int*>(full + kRingStages);
+        rows = rows_;
+        stage_rows = stage_rows_;
+        row_bytes = row_bytes_;
+        reverse = reverse_;
+        n = (rows + stage_rows - 1) / stage_rows;
+    }
+    // Rows [first, first + count) of stage i.
+    __device__ __forceinline__ int first(int i) const {
+        return reverse ? max(0, rows - (i + 1) * stage_rows) : i * stage_rows;
+    }
+    __device__ __forceinline__ int count(int i) const { return min(stage_rows, rows - i * stage_rows); }
+    __device__ __forceinline__ void issue(int i) {
+        const int slot = i % kRingStages;
+        const uint32_t bytes = uint32_t(count(i)) * uint32_t(row_bytes);
+        mbar_arrive_expect_tx(full + slot, NT * bytes);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            bulk_g2s(buf + slot * kRingStageBytes + t * kPart, src[t] + int64_t(first(i)) * row_bytes, bytes, full + slot);
+    }
+    // Before a block barrier; `issue` may follow it.
+    __device__ __forceinline__ void setup() {
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int k = 0; k < kRingStages; ++k) {
+                mbar_init(full + k, 1);
+                left[k] = 0;
+            }
+            mbar_fence_init();
+        }
+    }
+    __device__ __forceinline__ void fill() {
+        if (threadIdx.x == 0)
+            for (int i = 0; i < min(n, kRingStages); ++i) issue(i);
+    }
+    // use(stage's bytes, its first row, its rows)
+    template <typename F>
+    __device__ __forceinline__ void run(F use) {
+        for (int i = 0; i < n; ++i) {
+            const int slot = i % kRingStages;
+            if (!dead) dead = !mbar_wait_sleep(full + slot, uint32_t(i / kRingStages) & 1u, nullptr);
+            use(buf + slot * kRingStageBytes, first(i), count(i));
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0 && i + kRingStages < n) {
+                __threadfence_block();
+                if (atomicAdd(left + slot, 1) == kGnWarps - 1) {
+                    left[slot] = 0;
+                    __threadfence_block();
+                    fence_proxy_async_smem();
+                    issue(i + kRingStages);
+                }
+            }
+        }
+        if (dead)   // copies still in flight must not outlive the block
+            for (int k = 0; k < min(n, kRingStages); ++k) mbar_wait_sleep(full + k, uint32_t((n - 1 - k) / kRingStages) & 1u, nullptr);
+    }
+};
+
 // Mean (about the pivot) and M of the first `k` of U vectors of a thread, per
 // channel, or one for all channels of a vector that lies in one group: two
 // passes over the registers.  The sum of a batch of 16-bit values is taken as
@@ -370,28 +450,39 @@ struct Batch {
 };
 
 // Forward, sweep 1: moments of every group over a chunk.
-template <typename T, int VEC, bool ONEG>
+template <typename T, int VEC, bool ONEG, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ float gn_smem[];
-    constexpr int W = ONEG ? 1 : VEC, U = 8;
+    extern __shared__ __align__(16) float gn_smem[];
+    constexpr int W = ONEG ? 1 : VEC, U = RING ? 4 : 8;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G] mean, M of the tiles so far
-    float2* part = acc + G;                             // [rp][nv * W]
+    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
+    float2* acc = reinterpret_cast<float2*>(smem + (RING ? Ring<1>::bytes() : 0));   // [G] mean, M of the tiles so far
+    float2* part = RING ? reinterpret_cast<float2*>(smem) : acc + G;                 // [rp][nv * W], on the ring when it is done
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     pdl_launch_dependents();
+    Ring<1> ring;
+    if constexpr (RING) {
+        const Place pc(cv, 0);
+        ring.init(smem, p1 - p0, pc.rp * U, C * int(sizeof(T)), false);
+        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+        ring.setup();
+        __syncthreads();
+        ring.fill();
+    }
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
         const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
-        if (pc.on) {
+        float mean[W], m2[W];
+        {
             PerGroup<VEC, ONEG> pivot;
-            pivot.fill(c0 + pc.v * VEC, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
+            if (pc.on) pivot.fill(c0 + pc.v * VEC, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
             const T* xc = x + int64_t(p0 + pc.r) * a.xp + c0 + pc.v * VEC;
             const int64_t step = int64_t(pc.rp) * a.xp;
-            float n_run = 0.0f, mean[W], m2[W];
+            float n_run = 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) mean[j] = m2[j] = 0.0f;
             Batch<T, VEC, ONEG> bt;
@@ -405,22 +496,45 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
                 }
                 n_run = tot;
             };
-            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
-            for (; left >= U; left -= U) {
-                Pack<T, VEC> raw[U];
+            if constexpr (RING) {
+                ring.run([&](const unsigned char* sx, int, int rows) {
+                    const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + pc.v * VEC;
+                    const int k = pc.on ? (rows - pc.r + pc.rp - 1) / pc.rp : 0;
+                    Pack<T, VEC> raw[U];
+                    if (k == U) {
 #pragma unroll
-                for (int u = 0; u < U; ++u, xc += step) raw[u] = load_pack<T, VEC>(xc);
-                bt.template take<U, true>(raw, pivot, U);
-                join(float(U));
-            }
-            if (left > 0) {
-                Pack<T, VEC> raw[U];
+                        for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                        bt.template take<U, true>(raw, pivot, U);
+                        join(float(U));
+                    } else if (k > 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u, xc += step)
-                    if (u < left) raw[u] = load_pack<T, VEC>(xc);
-                bt.template take<U, false>(raw, pivot, left);
-                join(float(left));
+                        for (int u = 0; u < U; ++u)
+                            if (u < k) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                        bt.template take<U, false>(raw, pivot, k);
+                        join(float(k));
+                    }
+                });
+                if (ring.dead) mean[0] = __int_as_float(0x7fffffff);
+                __syncthreads();   // the ring's memory is the partials' from here on
+            } else if (pc.on) {
+                int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+                for (; left >= U; left -= U) {
+                    Pack<T, VEC> raw[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u, xc += step) raw[u] = load_pack<T, VEC>(xc);
+                    bt.template take<U, true>(raw, pivot, U);
+                    join(float(U));
+                }
+                if (left > 0) {
+                    Pack<T, VEC> raw[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u, xc += step)
+                        if (u < left) raw[u] = load_pack<T, VEC>(xc);
+                    bt.template take<U, false>(raw, pivot, left);
+                    join(float(left));
+                }
             }
+            if (pc.on)
 #pragma unroll
             for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(mean[j], m2[j]);
         }
@@ -457,18 +571,29 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
 }
 
 // Forward, sweep 2: merges the sample's chunks, writes y.
-template <typename T, int VEC, int ACT, bool ONEG>
+template <typename T, int VEC, int ACT, bool ONEG, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ float gn_smem[];
-    float2* st = reinterpret_cast<float2*>(gn_smem);   // [G] mean, rstd
-    constexpr int U = 8;
+    extern __shared__ __align__(16) float gn_smem[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
+    float2* st = reinterpret_cast<float2*>(smem + (RING ? Ring<1>::bytes() : 0));   // [G] mean, rstd
+    constexpr int U = RING ? 4 : 8;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
+    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     pdl_launch_dependents();
+    Ring<1> ring;
+    if constexpr (RING) {   // x is on its way while the partials are merged
+        const Place pc(cv, 0);
+        ring.init(smem, pv - p0, pc.rp * U, C * int(sizeof(T)), true);
+        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+        ring.setup();
+        __syncthreads();
+        ring.fill();
+    }
     pdl_wait();
     {
         __shared__ Merge merged[kGnWarps][32];
@@ -497,16 +622,27 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
             __syncthreads();
         }
     }
-    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        if (!pc.on) continue;
+        if (!RING && !pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
         Forward<T, VEC, ACT, ONEG> fw;
-        fw.load(a, c, c, Cg, st);
-        for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
+        if (pc.on) fw.load(a, c, c, Cg, st);
+        for (int p = pv + pc.r; pc.on && p < pe; p += pc.rp)   // padding
             store_pack<T, VEC>(y + int64_t(p) * C + c, pack_zero<T, VEC>());
+        if constexpr (RING) {
+            ring.run([&](const unsigned char* sx, int first, int rows) {
+                if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
+                const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + pc.v * VEC;
+                T* to = y + int64_t(p0 + first + pc.r) * C + c;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (pc.on && pc.r + u * pc.rp < rows)
+                        store_pack<T, VEC>(to + u * pc.rp * C, fw(load_pack<T, VEC>(at + u * pc.rp * C), a.act));
+            });
+            return;
+        }
         int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
         const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
         T* yc = y + int64_t(pv - 1 - pc.r) * C + c;
@@ -523,14 +659,15 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
 }
 
 // Backward, sweep 1: per-channel and per-group sums over a chunk.
-template <typename T, int VEC, int ACT, bool ONEG>
+template <typename T, int VEC, int ACT, bool ONEG, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ float gn_smem[];
-    constexpr int U = 4;
+    extern __shared__ __align__(16) float gn_smem[];
+    constexpr int U = RING ? 2 : 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G]
-    float2* part = acc + G;                             // [rp][nv * VEC]
+    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
+    float2* acc = reinterpret_cast<float2*>(smem + (RING ? Ring<2>::bytes() : 0));   // [G]
+    float2* part = RING ? reinterpret_cast<float2*>(smem) : acc + G;                 // [rp][nv * VEC], on the ring when it is done
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int64_t slot = int64_t(n) * pl.chunks + chunk;
     const int len = valid_len(a, n);
@@ -540,34 +677,58 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
     const float2* st = reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G;
     pdl_launch_dependents();
     for (int g = threadIdx.x; g < G; g += kGnThreads) acc[g] = make_float2(0.0f, 0.0f);
+    Ring<2> ring;
+    if constexpr (RING) {
+        const Place pc(cv, 0);
+        ring.init(smem, p1 - p0, pc.rp * U, C * int(sizeof(T)), false);
+        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+        ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
+        ring.setup();
+    }
     __syncthreads();
+    if constexpr (RING) ring.fill();
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
         const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
-        if (pc.on) {
+        {
             const int c = c0 + pc.v * VEC;
             Backward<T, VEC, ACT, ONEG> bw;
-            bw.load(a, c, c, Cg, st);
+            if (pc.on) bw.load(a, c, c, Cg, st);
             constexpr int NP = pairs_of(VEC);
             float2 sa[NP], sb[NP];
 #pragma unroll
             for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
-            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
-            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
-            const T* gc = dy + int64_t(p0 + pc.r) * a.gp + c;
-            const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp;
-            for (; left >= U; left -= U) {
-                Pack<T, VEC> rx[U], rg[U];
+            if constexpr (RING) {
+                ring.run([&](const unsigned char* s0, int, int rows) {
+                    const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + pc.v * VEC;
+                    const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + pc.v * VEC;
 #pragma unroll
-                for (int u = 0; u < U; ++u, xc += xs, gc += gs) {
-                    rx[u] = load_pack<T, VEC>(xc);
-                    rg[u] = load_pack<T, VEC>(gc);
+                    for (int u = 0; u < U; ++u)
+                        if (pc.on && pc.r + u * pc.rp < rows)
+                            bw.sums(load_pack<T, VEC>(sx + u * pc.rp * C), load_pack<T, VEC>(sg + u * pc.rp * C), a.act,
+                                    sa, sb);
+                });
+                if (ring.dead) sa[0] = splat2(__int_as_float(0x7fffffff));
+                __syncthreads();   // the ring's memory is the partials' from here on
+            } else if (pc.on) {
+                int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+                const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
+                const T* gc = dy + int64_t(p0 + pc.r) * a.gp + c;
+                const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp;
+                for (; left >= U; left -= U) {
+                    Pack<T, VEC> rx[U], rg[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u, xc += xs, gc += gs) {
+                        rx[u] = load_pack<T, VEC>(xc);
+                        rg[u] = load_pack<T, VEC>(gc);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
                 }
-#pragma unroll
-                for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
+                for (; left > 0; --left, xc += xs, gc += gs)
+                    bw.sums(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act, sa, sb);
             }
-            for (; left > 0; --left, xc += xs, gc += gs)
-                bw.sums(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act, sa, sb);
+            if (pc.on)
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
                 part[(pc.r * pc.nv + pc.v) * VEC + j] =
@@ -610,18 +771,32 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
 }
 
 // Backward, sweep 2: merges the sample's group sums, writes dx.
-template <typename T, int VEC, int ACT, bool ONEG>
+template <typename T, int VEC, int ACT, bool ONEG, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ float gn_smem[];
-    float4* gv = reinterpret_cast<float4*>(gn_smem);   // [G] mean, rstd, S1/m, S2/m
-    constexpr int U = 4;
+    extern __shared__ __align__(16) float gn_smem[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
+    float4* gv = reinterpret_cast<float4*>(smem + (RING ? (Ring<2>::bytes() + 15) / 16 * 16 : 0));   // [G] mean, rstd, S1/m, S2/m
+    constexpr int U = RING ? 2 : 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv = len > 0 ? 1.0f / (float(len) * float(Cg)) : 0.0f;
+    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
+    const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
+    const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
     pdl_launch_dependents();
+    Ring<2> ring;
+    if constexpr (RING) {   // x and dy are on their way while the partials are merged
+        const Place pc(cv, 0);
+        ring.init(smem, pv - p0, pc.rp * U, C * int(sizeof(T)), true);
+        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+        ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
+        ring.setup();
+        __syncthreads();
+        ring.fill();
+    }
     pdl_wait();
     {
         __shared__ float2 merged[kGnWarps][32];
@@ -649,19 +824,32 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
             __syncthreads();
         }
     }
-    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
-    const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
-    const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
     T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        if (!pc.on) continue;
+        if (!RING && !pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
         BackwardDx<T, VEC, ACT, ONEG> bw;
-        bw.load(a, c, c, Cg, gv);
-        bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
-        for (int p = pv + pc.r; p < pe; p += pc.rp)   // padding
+        if (pc.on) {
+            bw.load(a, c, c, Cg, gv);
+            bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
+        }
+        for (int p = pv + pc.r; pc.on && p < pe; p += pc.rp)   // padding
             store_pack<T, VEC>(dx + int64_t(p) * C + c, pack_zero<T, VEC>());
+        if constexpr (RING) {
+            ring.run([&](const unsigned char* s0, int first, int rows) {
+                if (ring.dead) bw.rw[0] = splat2(__int_as_float(0x7fffffff));
+                const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + pc.v * VEC;
+                const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + pc.v * VEC;
+                T* to = dx + int64_t(p0 + first + pc.r) * C + c;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (pc.on && pc.r + u * pc.rp < rows)
+                        store_pack<T, VEC>(to + u * pc.rp * C, bw.dx(load_pack<T, VEC>(sx + u * pc.rp * C),
+                                                                     load_pack<T, VEC>(sg + u * pc.rp * C), a.act));
+            });
+            return;
+        }
         int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
         const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
         const T* gc = dy + int64_t(pv - 1 - pc.r) * a.gp + c;
@@ -1024,27 +1212,35 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
     return rc ? rc : launch_params(pl, st);
 }
 
-template <typename T, int VEC, int ACT, bool ONEG>
+template <typename T, int VEC, int ACT, bool ONEG, bool RING>
 int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     const GroupNormArgs& a = pl.a;
     sweep_plan(pl);
     carve(ws, pl, backward);
-    const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
-    const size_t s1 = (size_t(a.G) + part) * sizeof(float2);
-    const size_t s2 = size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
+    const size_t base = RING ? (backward ? Ring<2>::bytes() : Ring<1>::bytes()) + 16 : 0;
+    const size_t part = RING ? 0 : size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
+    const size_t s1 = base + (size_t(a.G) + part) * sizeof(float2);
+    const size_t s2 = base + size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
     const int64_t blocks = a.N * pl.chunks;
     const bool second = !backward || a.dx != nullptr;
     int rc;
     {
         ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st, second ? 2 : 1);
-        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, false, st)
-                      : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, false, st);
+        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s1, 1, false, st)
+                      : launch(gn_moments_kernel<T, VEC, ONEG, RING>, pl, blocks, kGnThreads, s1, 1, false, st);
         if (!rc && second)
-            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st)
-                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, true, st);
+            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s2, 1, true, st)
+                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s2, 1, true, st);
     }
     if (rc) return rc;
     return backward ? launch_params(pl, st) : DOT_OK;
+}
+
+// Whether the sweeps take their rows by bulk copies: rows one after another in
+// memory, of whole 16-byte vectors, at most one per thread, and groups few
+// enough to leave the ring its shared memory.
+bool ring_rows(const GroupNormArgs& a, int vec, bool backward) {
+    return a.C / vec <= kGnThreads && a.G <= 1024 && a.xp == a.C && (!backward || a.gp == a.C);
 }
 
 template <typename T, int VEC, int ACT, bool ONEG>
@@ -1052,8 +1248,11 @@ int run(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st) {
     GnPlan pl{};
     pl.a = a;
     int threads, vecs;
-    if (!resident_plan(pl, VEC, sizeof(T), backward, threads, vecs))
-        return sweep_run<T, VEC, ACT, ONEG>(pl, ws, backward, st);
+    if (!resident_plan(pl, VEC, sizeof(T), backward, threads, vecs)) {
+        if constexpr (VEC * sizeof(T) == 16)
+            if (ring_rows(a, VEC, backward)) return sweep_run<T, VEC, ACT, ONEG, true>(pl, ws, backward, st);
+        return sweep_run<T, VEC, ACT, ONEG, false>(pl, ws, backward, st);
+    }
     constexpr int most = res_vecs(VEC * sizeof(T), true);
     if (vecs <= most / 4) return resident_run<T, VEC, ACT, ONEG, most / 4>(pl, ws, threads, backward, st);
     if (vecs <= most) return resident_run<T, VEC, ACT, ONEG, most>(pl, ws, threads, backward, st);
