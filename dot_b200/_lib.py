@@ -8,6 +8,8 @@ fails loudly -- there is no fallback implementation.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
@@ -100,6 +102,19 @@ def load() -> ctypes.CDLL:
         raise ImportError(f"dot_b200: library ABI {lib.dot_abi_version()} != expected {ABI_VERSION}")
     _lib = lib
     return lib
+
+
+def load_torch_binding():
+    """The torch binding of the feature operators (``_lib/_torch_features.so``)."""
+    path = os.path.join(_HERE, "_lib", "_torch_features.so")
+    if not os.path.exists(path):
+        raise ImportError(f"dot_b200: torch binding not found at {path}; build it with `python dot_b200/build.py`")
+    load()
+    loader = importlib.machinery.ExtensionFileLoader("_torch_features", path)
+    spec = importlib.util.spec_from_file_location("_torch_features", path, loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
 
 
 def exported_symbols() -> list[str]:

@@ -6,7 +6,10 @@ object per source under ``dot_b200/_lib/obj``) and links them into
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3``.  The CUDA runtime is
 linked statically so the library carries no dependency beyond the driver
 (NCCL, used only by the row-sharded solver, is loaded at run time).
-The build is skipped when the library is newer than every source.
+``csrc/torch_features.cpp``, the torch binding of the feature operators, is
+compiled with the host compiler against the installed torch and linked to that
+library (``_lib/_torch_features.so``).  Each is skipped when it is newer than
+its sources.
 """
 
 from __future__ import annotations
@@ -22,6 +25,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIB_DIR, "libdot_b200.so")
+BINDING = os.path.join(LIB_DIR, "_torch_features.so")
+BINDING_SRC = os.path.join(HERE, "csrc", "torch_features.cpp")
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
 
@@ -45,9 +50,42 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """The torch binding: host code only, linked to libdot_b200.so beside it."""
+    deps = [BINDING_SRC, os.path.join(ROOT, "include", "dot_b200.h")]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    tmp = BINDING + ".tmp"
+    # the system compiler, whose C++ library the process runs on (not $CXX, which may bring another)
+    cmd = ["/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           "-DTORCH_EXTENSION_NAME=_torch_features",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += ["-I" + p for p in cpp_extension.include_paths() + [sysconfig.get_paths()["include"],
+                                                                os.path.join(cuda, "include")]]
+    cmd += [BINDING_SRC, "-o", tmp, "-L" + LIB_DIR, "-l:libdot_b200.so", "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-L" + p for p in cpp_extension.library_paths()]
+    cmd += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _stale():
-        return LIB
+    if force or _stale():
+        _build_library(verbose)
+    build_binding(force, verbose)
+    return LIB
+
+
+def _build_library(verbose: bool) -> None:
     obj_dir = os.path.join(LIB_DIR, "obj")
     os.makedirs(obj_dir, exist_ok=True)
     flags = [ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -70,7 +108,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":

@@ -253,20 +253,18 @@ def _rows(x: torch.Tensor):
     S = x.numel() // (N * C)
     if x.is_contiguous():
         return x, N, S, C, S * C, C
-    one, step = x.stride(-1), 0
+    step = after = None    # the positions' stride; the stride that continues the axes seen so far
     for size, stride in zip(reversed(x.shape[1:-1]), reversed(x.stride()[1:-1])):
         if size == 1:
             continue
-        if step == 0:
-            step, span = stride, stride * size
-        elif stride != span:
-            step = -1
-            break
-        else:
-            span = stride * size
-    if step < 0 or (C > 1 and one != 1):
+        if step is None:
+            step = stride
+        elif stride != after:
+            return x.contiguous(), N, S, C, S * C, C
+        after = stride * size
+    if C > 1 and x.stride(-1) != 1:
         return x.contiguous(), N, S, C, S * C, C
-    return x, N, S, C, x.stride(0), step
+    return x, N, S, C, x.stride(0), step or 0
 
 
 @functools.lru_cache(maxsize=1024)

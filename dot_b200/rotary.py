@@ -11,59 +11,20 @@ positions.  The axes may be row and column of an image, time, height and width
 of a clip, or the coordinates of a keypoint; a row of ``freqs`` with one
 non-zero entry gives a pair to one axis (:func:`rotary_freqs` builds such
 tables), a full row mixes the axes.  Queries and keys with different numbers
-of heads are turned in one launch; a single token is an ordinary call.  The
-reference has no such operator.
+of heads are turned in one launch; a single token is an ordinary call.  Checks,
+allocation and autograd are in ``csrc/torch_features.cpp``;
+:func:`dot_b200.ops.rotary_raw` is a single call of the C-ABI.  The reference
+has no such operator.
 """
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Sequence
 
 import torch
 import torch.nn as nn
 
-from . import ops
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved: bool, inverse: bool):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, freqs)
-        ctx.flags = (interleaved, inverse)
-        return ops.rotary_raw(q, k, positions, freqs, interleaved, inverse)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        need = ctx.needs_input_grad
-        if not need[0]:
-            dq = None
-        if not need[1]:
-            dk = None
-        if dq is None and dk is None:
-            return (None,) * 6
-        positions, freqs = ctx.saved_tensors
-        interleaved, inverse = ctx.flags
-        # the turn is orthogonal: its backward is the turn by -angle
-        turn = _RotaryFn.apply if torch.is_grad_enabled() else ops.rotary_raw
-        dq, dk = turn(dq, dk, positions, freqs, interleaved, not inverse)
-        return dq, dk, None, None, None, None
-
-
-def _check_heads(x: torch.Tensor, name: str) -> None:
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError(f"dot_b200: {name} must be a CUDA tensor (dot_b200 runs on NVIDIA GPUs only)")
-    if x.dim() < 3:
-        raise ValueError(f"{name} must be [..., tokens, heads, head_dim]")
-    if x.dtype not in ops._FEATURE_DTYPES:
-        raise NotImplementedError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
-
-
-def _as_4d(x: torch.Tensor) -> torch.Tensor:
-    if x.dim() == 3:
-        return x.unsqueeze(0)
-    return x.reshape(math.prod(x.shape[:-3]), *x.shape[-3:])
+from .norm import _binding
 
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Optional[torch.Tensor] = None,
@@ -77,47 +38,8 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Opt
     (a fused projection); the results are dense.  Returns q', or (q', k') when
     k is given.  Differentiable in q and k, not in positions or freqs.
     """
-    _check_heads(q, "q")
-    shape = q.shape
-    lead = shape[:-2]
-    grad = q.requires_grad
-    if k is not None:
-        _check_heads(k, "k")
-        if k.shape[:-2] != lead or k.size(-1) != shape[-1]:
-            raise ValueError("k must have q's shape except for the number of heads")
-        if k.dtype != q.dtype or k.get_device() != q.get_device():
-            raise ValueError("k must have q's dtype and device")
-        grad = grad or k.requires_grad
-    if freqs.dim() != 2 or freqs.dtype != torch.float32:
-        raise ValueError("freqs must be float32 [P, A]")
-    if positions.dtype not in ops._POSITION_DTYPES:
-        raise ValueError("positions must be int32, int64 or float32")
-    if positions.get_device() != q.get_device() or freqs.get_device() != q.get_device():
-        raise ValueError("positions and freqs must be on q's device")
-    if positions.requires_grad or freqs.requires_grad:
-        raise ValueError("positions and freqs are not differentiable here: detach them")
-    P, A = freqs.shape
-    if not 1 <= A <= 4:
-        raise ValueError("freqs must have 1 to 4 axes")
-    if 2 * P > shape[-1]:
-        raise ValueError("freqs must hold at most D/2 pairs")
-    if positions.shape != (*lead, A):
-        if positions.shape != (lead[-1], A):
-            raise ValueError("positions must be [*, L, A] with q's leading axes, or [L, A]")
-        positions = positions.unsqueeze(0)
-    elif len(lead) != 2:
-        positions = positions.reshape(math.prod(lead[:-1]), lead[-1], A)
-    if not freqs.is_contiguous():
-        freqs = freqs.contiguous()
-    q4, k4 = (q, k) if len(lead) == 2 else (_as_4d(q), None if k is None else _as_4d(k))
-    if grad and torch.is_grad_enabled():
-        q4, k4 = _RotaryFn.apply(q4, k4, positions, freqs, bool(interleaved), False)
-    else:
-        q4, k4 = ops.rotary_raw(q4, k4, positions, freqs, bool(interleaved))
-    if len(lead) != 2:
-        q4 = q4.view(shape)
-        k4 = None if k is None else k4.view(k.shape)
-    return q4 if k is None else (q4, k4)
+    q, turned_k = _binding.rotary(q, positions, freqs, k, interleaved)
+    return q if k is None else (q, turned_k)
 
 
 def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, shared_band: bool = False,

@@ -418,3 +418,40 @@ def test_refusals():
         y = dot.group_norm_act(x.requires_grad_(True), 4)
         (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("shape,expand", [((2, 5, 1, 16), (2, 5, 7, 16)), ((2, 1, 7, 16), (2, 5, 7, 16)),
+                                          ((1, 5, 7, 16), (2, 5, 7, 16)), ((2, 1, 1, 16), (2, 5, 7, 16)),
+                                          ((2, 5, 7, 1), (2, 5, 7, 16))])
+def test_expanded_axes(shape, expand):
+    """Inputs and gradients repeated along some axes (strides of 0) give what their copies give."""
+    x, g = (torch.randn(shape, generator=U.gen(k)).to(DEV).expand(expand) for k in (1, 2))
+    outs = []
+    for a, b in ((x, g), (x.contiguous(), g.contiguous())):
+        leaf = a.detach().requires_grad_(True)
+        y = dot.group_norm_act(leaf, 4)
+        outs.append((y.detach(), torch.autograd.grad(y, leaf, b)[0]))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("shape", [(2, 5000, 64), (1, 30, 24), (2, 4, 9, 15)])
+def test_single_calls_of_the_c_abi(shape):
+    """dot_b200.ops' raw functions and the public operator are the same calls."""
+    from dot_b200 import ops
+
+    x, dy = (torch.randn(shape, generator=U.gen(k)).to(DEV) for k in (1, 2))
+    w, b = (torch.randn(shape[-1], generator=U.gen(k)).to(DEV) for k in (3, 4))
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = dot.group_norm_act(leaves[0], 1, leaves[1], leaves[2], activation="gelu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    y2, stats = ops.group_norm_forward_raw(x, 1, w, b, 1e-5, 2)
+    assert torch.equal(y, y2)
+    for got, want in zip(ops.group_norm_backward_raw(x, dy, 1, w, b, 2, stats), grads):
+        assert torch.equal(got, want)
+
+
+def test_a_recorded_backward_is_not_differentiated_again():
+    x = torch.randn(2, 10, 16, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(dot.group_norm_act(x, 4).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        (g.sum() + x.sum()).backward()

@@ -294,3 +294,15 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="4096"):
         dot.rotary(torch.zeros(1, 1, 8194, device=DEV), torch.zeros(1, 1, device=DEV),
                    torch.zeros(4097, 1, device=DEV))
+
+
+def test_single_calls_of_the_c_abi():
+    """dot_b200.ops.rotary_raw and the public operator are the same call."""
+    from dot_b200 import ops
+
+    q, k, freqs = rand(2, 30, 4, 40, seed=1), rand(2, 30, 2, 40, seed=2), table(16, 2)
+    pos = torch.randint(0, 60, (30, 2), generator=U.gen(2)).to(DEV)
+    want = dot.rotary(q, pos, freqs, k=k)
+    got = ops.rotary_raw(q, k, pos.unsqueeze(0), freqs, False)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(ops.rotary_raw(None, k, pos.unsqueeze(0), freqs, False)[1], want[1])
