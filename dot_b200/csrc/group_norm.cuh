@@ -251,30 +251,33 @@ struct BackwardDx : Backward<T, VEC, ACT, ONEG> {
 };
 
 // ---- backward: the parameters' gradients from the blocks' channel sums ---------
-__global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
+
+// Channels c = first + warp, + kGnWarps, ... < end: a warp sums a channel's
+// pairs over all samples' chunks, in an order that depends on nothing else.
+__device__ __forceinline__ void param_grads(const GnPlan& pl, int first, int end) {
     const GroupNormArgs& a = pl.a;
-    __shared__ float2 part[kGnWarps][32];
-    const int C = int(a.C), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
+    const int C = int(a.C), lane = threadIdx.x & 31;
     const int64_t rows = a.N * pl.chunks;
-    float2 s = make_float2(0.0f, 0.0f);
-    if (c < C)
-#pragma unroll 8
-        for (int64_t r = warp; r < rows; r += kGnWarps) {
+    for (int c = first + int(threadIdx.x >> 5); c < end; c += kGnWarps) {
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+        for (int64_t r = lane; r < rows; r += 32) {
             const float2 v = pl.csums[r * C + c];
             s.x += v.x;
             s.y += v.y;
         }
-    part[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0 && c < C) {
-        for (int k = 1; k < kGnWarps; ++k) {
-            s.x += part[k][lane].x;
-            s.y += part[k][lane].y;
+        s = lanes_sum(s, 5);
+        if (lane == 0) {
+            if (a.dbias) store_param(a.dbias, a.param_dtype, c, s.x);
+            if (a.dweight) store_param(a.dweight, a.param_dtype, c, s.y);
         }
-        if (a.dbias) store_param(a.dbias, a.param_dtype, c, s.x);
-        if (a.dweight) store_param(a.dweight, a.param_dtype, c, s.y);
     }
+}
+
+// A launch of its own where no other one follows the sums.
+__global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
+    pdl_wait();
+    param_grads(pl, int(blockIdx.x) * kGnWarps, min(int(pl.a.C), int(blockIdx.x + 1) * kGnWarps));
 }
 
 // ---- two sweeps per direction --------------------------------------------------
@@ -301,8 +304,8 @@ struct Place {
     }
 };
 
-// A ring of bulk copies for rows that lie one after another in memory: 192 KB
-// in flight per SM without a register.  A stage holds U rows for each row
+// A ring of bulk copies for rows that lie one after another in memory: up to
+// 192 KB in flight per SM without a register.  A stage holds U rows for each row
 // position of the block, of x and for NT = 2 of dy; the last of the 16 warps to
 // leave a stage refills it.  Waits are bounded: one that expires makes the
 // block go on without waiting, and its results are written as NaN.
@@ -319,7 +322,9 @@ struct Ring {
     int row_bytes, rows, stage_rows, n; // rows in all, per stage; stages
     bool reverse, dead = false;
 
-    static constexpr size_t bytes() { return size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + sizeof(int)); }
+    static constexpr size_t bytes() {   // what follows is 16-byte aligned
+        return (size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + sizeof(int)) + 15) / 16 * 16;
+    }
     __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_, bool reverse_) {
         buf = smem;
         full = reinterpret_cast<uint64_t*>(smem + kRingStages * kRingStageBytes);
@@ -776,7 +781,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ __align__(16) float gn_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
-    float4* gv = reinterpret_cast<float4*>(smem + (RING ? (Ring<2>::bytes() + 15) / 16 * 16 : 0));   // [G] mean, rstd, S1/m, S2/m
+    float4* gv = reinterpret_cast<float4*>(smem + (RING ? Ring<2>::bytes() : 0));   // [G] mean, rstd, S1/m, S2/m
     constexpr int U = RING ? 2 : 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
@@ -798,6 +803,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
         ring.fill();
     }
     pdl_wait();
+    if (a.dweight || a.dbias) {   // the blocks share out the channels while their first rows arrive
+        const int per = (C + int(gridDim.x) - 1) / int(gridDim.x);
+        param_grads(pl, int(blockIdx.x) * per, min(C, int(blockIdx.x + 1) * per));
+    }
     {
         __shared__ float2 merged[kGnWarps][32];
         const int parts = pl.chunks;
@@ -987,6 +996,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan p
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
     const int C = int(a.C), G = int(a.G), Cg = C / G;
+    pdl_launch_dependents();
     const ResPlace pc(pl, Cg, VEC);
     float2* sums = reinterpret_cast<float2*>(gn_smem);   // [slab_groups] S1/m, S2/m
     float2* mine = sums + pl.slab_groups;                // [slab_groups] this block's S1, S2
@@ -1160,7 +1170,7 @@ int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem,
 int launch_params(const GnPlan& pl, cudaStream_t st) {
     if (!pl.a.dweight && !pl.a.dbias) return DOT_OK;
     ProfScope ps(DOT_K_NORM_BWD, st);
-    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, 32), kGnThreads, 0, 1, false, st);
+    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, kGnWarps), kGnThreads, 0, 1, true, st);
 }
 
 // The resident plan of a problem, if its blocks hold it in registers all at
@@ -1217,7 +1227,7 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     const GroupNormArgs& a = pl.a;
     sweep_plan(pl);
     carve(ws, pl, backward);
-    const size_t base = RING ? (backward ? Ring<2>::bytes() : Ring<1>::bytes()) + 16 : 0;
+    const size_t base = RING ? (backward ? Ring<2>::bytes() : Ring<1>::bytes()) : 0;
     const size_t part = RING ? 0 : size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
     const size_t s1 = base + (size_t(a.G) + part) * sizeof(float2);
     const size_t s2 = base + size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
@@ -1233,7 +1243,7 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
                           : launch(gn_apply_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s2, 1, true, st);
     }
     if (rc) return rc;
-    return backward ? launch_params(pl, st) : DOT_OK;
+    return backward && !second ? launch_params(pl, st) : DOT_OK;
 }
 
 // Whether the sweeps take their rows by bulk copies: rows one after another in
