@@ -24,6 +24,8 @@
 // (Chan, Golub and LeVeque, 1979); threads' and blocks' pairs are joined by Merge.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "cluster.cuh"
 #include "feature.cuh"
 #include "feature_ops.h"
@@ -262,7 +264,7 @@ __device__ __forceinline__ void param_grads(const GnPlan& pl, int first, int end
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 4
         for (int64_t r = lane; r < rows; r += 32) {
-            const float2 v = pl.csums[r * C + c];
+            const float2 v = __ldcg(pl.csums + r * C + c);
             s.x += v.x;
             s.y += v.y;
         }
@@ -304,12 +306,14 @@ struct Place {
     }
 };
 
-// A ring of bulk copies for rows that lie one after another in memory: up to
-// 192 KB in flight per SM without a register.  A stage holds U rows for each row
-// position of the block, of x and for NT = 2 of dy; the last of the 16 warps to
-// leave a stage refills it.  Waits are bounded: one that expires makes the
-// block go on without waiting, and its results are written as NaN.
-constexpr int kRingStages = 6;
+// A ring of bulk copies for rows that lie one after another in memory, walked
+// forwards and then backwards: up to 160 KB in flight per SM without a
+// register, and the way back begins with the stages that are still there.  A
+// stage holds U rows for each row position of the block, of x and for NT = 2 of
+// dy; the last of the 16 warps to leave a stage refills it.  Waits are bounded:
+// one that expires makes the block go on without waiting, and its results are
+// written as NaN.
+constexpr int kRingStages = 5;
 constexpr int kRingStageBytes = 32 * 1024;
 
 template <int NT>
@@ -320,36 +324,20 @@ struct Ring {
     int* left;                          // [kRingStages] warps that have left the stage
     const unsigned char* src[NT];       // row 0 of the block's range
     int row_bytes, rows, stage_rows, n; // rows in all, per stage; stages
-    bool reverse, dead = false;
+    bool dead = false;
 
     static constexpr size_t bytes() {   // what follows is 16-byte aligned
         return (size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + sizeof(int)) + 15) / 16 * 16;
     }
-    __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_, bool reverse_) {
+    // By all threads, before a block barrier.
+    __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_) {
         buf = smem;
         full = reinterpret_cast<uint64_t*>(smem + kRingStages * kRingStageBytes);
         left = reinterpret_cast<int*>(full + kRingStages);
         rows = rows_;
         stage_rows = stage_rows_;
         row_bytes = row_bytes_;
-        reverse = reverse_;
         n = (rows + stage_rows - 1) / stage_rows;
-    }
-    // Rows [first, first + count) of stage i.
-    __device__ __forceinline__ int first(int i) const {
-        return reverse ? max(0, rows - (i + 1) * stage_rows) : i * stage_rows;
-    }
-    __device__ __forceinline__ int count(int i) const { return min(stage_rows, rows - i * stage_rows); }
-    __device__ __forceinline__ void issue(int i) {
-        const int slot = i % kRingStages;
-        const uint32_t bytes = uint32_t(count(i)) * uint32_t(row_bytes);
-        mbar_arrive_expect_tx(full + slot, NT * bytes);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            bulk_g2s(buf + slot * kRingStageBytes + t * kPart, src[t] + int64_t(first(i)) * row_bytes, bytes, full + slot);
-    }
-    // Before a block barrier; `issue` may follow it.
-    __device__ __forceinline__ void setup() {
         if (threadIdx.x == 0) {
 #pragma unroll
             for (int k = 0; k < kRingStages; ++k) {
@@ -359,30 +347,60 @@ struct Ring {
             mbar_fence_init();
         }
     }
+    // Stage i holds rows [i stage_rows, + count(i)).
+    __device__ __forceinline__ int count(int i) const { return min(stage_rows, rows - i * stage_rows); }
+    __device__ __forceinline__ void issue(int i) {
+        const int slot = i % kRingStages;
+        const uint32_t bytes = uint32_t(count(i)) * uint32_t(row_bytes);
+        mbar_arrive_expect_tx(full + slot, NT * bytes);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            bulk_g2s(buf + slot * kRingStageBytes + t * kPart, src[t] + int64_t(i) * stage_rows * row_bytes, bytes,
+                     full + slot);
+    }
+    // After that barrier.
     __device__ __forceinline__ void fill() {
         if (threadIdx.x == 0)
             for (int i = 0; i < min(n, kRingStages); ++i) issue(i);
     }
-    // use(stage's bytes, its first row, its rows)
+    // A warp leaves stage i; the last one brings stage `next` into its place.
+    __device__ __forceinline__ void leave(int i, int next) {
+        const int slot = i % kRingStages;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            __threadfence_block();
+            if (atomicAdd(left + slot, 1) == kGnWarps - 1) {
+                left[slot] = 0;
+                __threadfence_block();
+                fence_proxy_async_smem();
+                issue(next);
+            }
+        }
+    }
+    // use(stage's bytes, its first row, its rows), first stage to last.  The
+    // c-th copy into a slot completes its barrier's phase c: stage i is copy
+    // i / kRingStages of its slot on the way forwards ...
     template <typename F>
-    __device__ __forceinline__ void run(F use) {
+    __device__ __forceinline__ void forwards(F use) {
         for (int i = 0; i < n; ++i) {
             const int slot = i % kRingStages;
             if (!dead) dead = !mbar_wait_sleep(full + slot, uint32_t(i / kRingStages) & 1u, nullptr);
-            use(buf + slot * kRingStageBytes, first(i), count(i));
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0 && i + kRingStages < n) {
-                __threadfence_block();
-                if (atomicAdd(left + slot, 1) == kGnWarps - 1) {
-                    left[slot] = 0;
-                    __threadfence_block();
-                    fence_proxy_async_smem();
-                    issue(i + kRingStages);
-                }
-            }
+            use(buf + slot * kRingStageBytes, i * stage_rows, count(i));
+            if (i + kRingStages < n) leave(i, i + kRingStages);
         }
-        if (dead)   // copies still in flight must not outlive the block
-            for (int k = 0; k < min(n, kRingStages); ++k) mbar_wait_sleep(full + k, uint32_t((n - 1 - k) / kRingStages) & 1u, nullptr);
+    }
+    // ... and, m = (slot's last stage) / kRingStages, copy 2 m - i / kRingStages
+    // on the way back, which has the same parity.  The last stages are still there.
+    template <typename F>
+    __device__ __forceinline__ void backwards(F use) {
+        for (int i = n - 1; i >= 0; --i) {
+            const int slot = i % kRingStages;
+            if (!dead && i < n - kRingStages) dead = !mbar_wait_sleep(full + slot, uint32_t(i / kRingStages) & 1u, nullptr);
+            use(buf + slot * kRingStageBytes, i * stage_rows, count(i));
+            if (i >= kRingStages) leave(i, i - kRingStages);
+        }
+        if (dead)   // copies still in flight must not outlive the block; the last into a slot is an even one
+            for (int k = 0; k < min(n, kRingStages); ++k) mbar_wait_sleep(full + k, 0u, nullptr);
     }
 };
 
@@ -454,121 +472,217 @@ struct Batch {
     }
 };
 
+// Joins a batch's pairs to a thread's running ones.
+template <typename T, int VEC, bool ONEG>
+struct Running {
+    static constexpr int W = ONEG ? 1 : VEC;
+    float n = 0.0f, mean[W], m2[W];
+    __device__ __forceinline__ Running() {
+#pragma unroll
+        for (int j = 0; j < W; ++j) mean[j] = m2[j] = 0.0f;
+    }
+    __device__ __forceinline__ void join(const Batch<T, VEC, ONEG>& b, float k) {
+        const float tot = n + k, f = __fdividef(k, tot), w = n * f * float(VEC / W);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const float d = b.mean[j] - mean[j];
+            mean[j] += d * f;
+            m2[j] += b.m2[j] + d * d * w;
+        }
+        n = tot;
+    }
+};
+
+// A tile's groups from its threads' pairs `part` [rp][nv * W] over `rows`
+// positions, joined to what earlier tiles left of them in acc [G].
+template <int VEC, int W>
+__device__ __forceinline__ void tile_moments(const Place& pc, int tile, int Cg, int rows, const float2* part, float2* acc) {
+    const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
+    const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
+    const int lane = int(threadIdx.x) & ((1 << log) - 1), full = rows / pc.rp;
+    for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
+        const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
+        const bool mine = gi < gn;
+        const int ca = max(c0, g * Cg), before = ca - g * Cg;   // channels of the group in earlier tiles
+        const int wd = (min(c1, (g + 1) * Cg) - ca) / (VEC / W), at = (ca - c0) / (VEC / W);
+        const float2 old = mine ? acc[g] : make_float2(0.0f, 0.0f);
+        const float about = mine ? part[at].x : 0.0f;   // row 0 is there if any is
+        Merge m;
+        if (mine) {
+            for (int i = lane; i < pc.rp * wd; i += 1 << log) {
+                const int r = wd == 1 ? i : i / wd;
+                const float2 v = part[r * pc.nv * W + at + i - r * wd];
+                const int cnt = full + (r < rows - full * pc.rp ? 1 : 0);
+                m.add(about, float(cnt * (VEC / W)), v.x, v.y);
+            }
+            if (before > 0 && lane == 0) m.add(about, float(rows) * float(before), old.x, old.y);
+        }
+        m.lanes(log);
+        __syncwarp();
+        if (mine && lane == 0) acc[g] = m.pair(about, float(rows) * float(min(c1, (g + 1) * Cg) - g * Cg));
+    }
+}
+
+// Statistics [G] of sample n from its chunks' moments, by the whole block.
+template <typename T>
+__device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write, int len, const T* x, float2* st) {
+    __shared__ Merge merged[kGnWarps][32];
+    const GroupNormArgs& a = pl.a;
+    const int G = int(a.G), Cg = int(a.C) / G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the chunks
+        Merge m;
+        const float2* from = pl.moments + int64_t(n) * pl.chunks * G + g;
+        const float about = g < G ? __ldcg(from).x : 0.0f;
+        if (g < G)
+#pragma unroll 8
+            for (int k = warp; k < pl.chunks; k += kGnWarps) {
+                const float2 v = __ldcg(from + int64_t(k) * G);
+                m.add(about, float(rows_of(len, k, pl.rows)) * float(Cg), v.x, v.y);
+            }
+        merged[warp][lane] = m;
+        __syncthreads();
+        if (warp == 0 && g < G) {
+#pragma unroll
+            for (int k = 1; k < kGnWarps; ++k) {
+                m.nd += merged[k][lane].nd;
+                m.m2 += merged[k][lane].m2;
+            }
+            st[g] = mean_rstd(group_pivot(x, len, g * Cg), m.pair(about, float(len) * float(Cg)), len, Cg, a.eps);
+            if (write) reinterpret_cast<float2*>(a.stats)[int64_t(n) * G + g] = st[g];
+        }
+        __syncthreads();
+    }
+}
+
+// A tile's channel sums (into the workspace's row `slot`) and, weighted, its
+// groups' (added to acc [G]) from its threads' pairs `part` [rp][nv * VEC].
+template <int VEC>
+__device__ __forceinline__ void tile_sums(const GnPlan& pl, const Place& pc, int tile, int64_t slot, float2* part, float2* acc) {
+    const GroupNormArgs& a = pl.a;
+    const int C = int(a.C), Cg = C / int(a.G), c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
+    for (int i = threadIdx.x; i < pc.nv * VEC; i += kGnThreads) {   // rows of a channel, in order
+        float2 s = part[i];
+        for (int r = 1; r < pc.rp; ++r) {
+            const float2 v = part[r * pc.nv * VEC + i];
+            s.x += v.x;
+            s.y += v.y;
+        }
+        part[i] = s;
+        pl.csums[slot * C + c0 + i] = s;
+    }
+    __syncthreads();
+    const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
+    const int lane = int(threadIdx.x) & ((1 << log) - 1);
+    for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
+        const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
+        float2 s = make_float2(0.0f, 0.0f);
+        if (gi < gn)
+            for (int c = max(c0, g * Cg) + lane; c < min(c1, (g + 1) * Cg); c += 1 << log) {
+                const float w = a.weight ? load_param(a.weight, a.param_dtype, c) : 1.0f;
+                s.x += w * part[c - c0].x;
+                s.y += w * part[c - c0].y;
+            }
+        s = lanes_sum(s, log);
+        if (gi < gn && lane == 0) {
+            acc[g].x += s.x;
+            acc[g].y += s.y;
+        }
+    }
+}
+
+// Mean, rstd, S1/m and S2/m [G] of sample n from its chunks' sums, by the whole
+// block; the blocks of the launch share out the parameters' gradients.
+__device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, float4* gv) {
+    __shared__ float2 merged[kGnWarps][32];
+    const GroupNormArgs& a = pl.a;
+    const int C = int(a.C), G = int(a.G), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float inv = len > 0 ? 1.0f / (float(len) * float(C / G)) : 0.0f;
+    if (a.dweight || a.dbias) {
+        const int per = (C + int(gridDim.x) - 1) / int(gridDim.x);
+        param_grads(pl, int(blockIdx.x) * per, min(C, int(blockIdx.x + 1) * per));
+    }
+    for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the chunks
+        float2 s = make_float2(0.0f, 0.0f);
+        if (g < G)
+#pragma unroll 8
+            for (int k = warp; k < pl.chunks; k += kGnWarps) {
+                const float2 v = __ldcg(pl.gsums + (int64_t(n) * pl.chunks + k) * G + g);
+                s.x += v.x;
+                s.y += v.y;
+            }
+        merged[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && g < G) {
+#pragma unroll
+            for (int k = 1; k < kGnWarps; ++k) {
+                s.x += merged[k][lane].x;
+                s.y += merged[k][lane].y;
+            }
+            const float2 v = reinterpret_cast<const float2*>(a.stats)[int64_t(n) * G + g];
+            gv[g] = make_float4(v.x, v.y, s.x * inv, s.y * inv);
+        }
+        __syncthreads();
+    }
+}
+
+// Zeros at a chunk's positions from pv on.
+template <typename T, int VEC>
+__device__ __forceinline__ void pad_rows(const Place& pc, T* out, int C, int c, int pv, int pe) {
+    for (int p = pv + pc.r; pc.on && p < pe; p += pc.rp) store_pack<T, VEC>(out + int64_t(p) * C + c, pack_zero<T, VEC>());
+}
+
+template <int VEC>
+__device__ __forceinline__ void put_pairs(float2* part, const float2* sa, const float2* sb) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        part[j] = j % 2 ? make_float2(sa[j / 2].y, sb[j / 2].y) : make_float2(sa[j / 2].x, sb[j / 2].x);
+}
+
 // Forward, sweep 1: moments of every group over a chunk.
-template <typename T, int VEC, bool ONEG, bool RING>
+template <typename T, int VEC, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ __align__(16) float gn_smem[];
-    constexpr int W = ONEG ? 1 : VEC, U = RING ? 4 : 8;
+    extern __shared__ float gn_smem[];
+    constexpr int W = ONEG ? 1 : VEC, U = 8;
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
-    float2* acc = reinterpret_cast<float2*>(smem + (RING ? Ring<1>::bytes() : 0));   // [G] mean, M of the tiles so far
-    float2* part = RING ? reinterpret_cast<float2*>(smem) : acc + G;                 // [rp][nv * W], on the ring when it is done
+    float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G] mean, M of the tiles so far
+    float2* part = acc + G;                             // [rp][nv * W]
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     pdl_launch_dependents();
-    Ring<1> ring;
-    if constexpr (RING) {
-        const Place pc(cv, 0);
-        ring.init(smem, p1 - p0, pc.rp * U, C * int(sizeof(T)), false);
-        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
-        ring.setup();
-        __syncthreads();
-        ring.fill();
-    }
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
-        float mean[W], m2[W];
-        {
+        const int c = (tile * kGnThreads + pc.v) * VEC;
+        if (pc.on) {
             PerGroup<VEC, ONEG> pivot;
-            if (pc.on) pivot.fill(c0 + pc.v * VEC, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
-            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c0 + pc.v * VEC;
+            pivot.fill(c, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
+            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
             const int64_t step = int64_t(pc.rp) * a.xp;
-            float n_run = 0.0f;
-#pragma unroll
-            for (int j = 0; j < W; ++j) mean[j] = m2[j] = 0.0f;
+            Running<T, VEC, ONEG> run;
             Batch<T, VEC, ONEG> bt;
-            auto join = [&](float k) {
-                const float tot = n_run + k, f = __fdividef(k, tot), w = n_run * f * float(VEC / W);
+            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+            for (; left >= U; left -= U) {
+                Pack<T, VEC> raw[U];
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const float d = bt.mean[j] - mean[j];
-                    mean[j] += d * f;
-                    m2[j] += bt.m2[j] + d * d * w;
-                }
-                n_run = tot;
-            };
-            if constexpr (RING) {
-                ring.run([&](const unsigned char* sx, int, int rows) {
-                    const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + pc.v * VEC;
-                    const int k = pc.on ? (rows - pc.r + pc.rp - 1) / pc.rp : 0;
-                    Pack<T, VEC> raw[U];
-                    if (k == U) {
-#pragma unroll
-                        for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
-                        bt.template take<U, true>(raw, pivot, U);
-                        join(float(U));
-                    } else if (k > 0) {
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-                            if (u < k) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
-                        bt.template take<U, false>(raw, pivot, k);
-                        join(float(k));
-                    }
-                });
-                if (ring.dead) mean[0] = __int_as_float(0x7fffffff);
-                __syncthreads();   // the ring's memory is the partials' from here on
-            } else if (pc.on) {
-                int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
-                for (; left >= U; left -= U) {
-                    Pack<T, VEC> raw[U];
-#pragma unroll
-                    for (int u = 0; u < U; ++u, xc += step) raw[u] = load_pack<T, VEC>(xc);
-                    bt.template take<U, true>(raw, pivot, U);
-                    join(float(U));
-                }
-                if (left > 0) {
-                    Pack<T, VEC> raw[U];
-#pragma unroll
-                    for (int u = 0; u < U; ++u, xc += step)
-                        if (u < left) raw[u] = load_pack<T, VEC>(xc);
-                    bt.template take<U, false>(raw, pivot, left);
-                    join(float(left));
-                }
+                for (int u = 0; u < U; ++u, xc += step) raw[u] = load_pack<T, VEC>(xc);
+                bt.template take<U, true>(raw, pivot, U);
+                run.join(bt, float(U));
             }
-            if (pc.on)
+            if (left > 0) {
+                Pack<T, VEC> raw[U];
 #pragma unroll
-            for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(mean[j], m2[j]);
+                for (int u = 0; u < U; ++u, xc += step)
+                    if (u < left) raw[u] = load_pack<T, VEC>(xc);
+                bt.template take<U, false>(raw, pivot, left);
+                run.join(bt, float(left));
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(run.mean[j], run.m2[j]);
         }
         __syncthreads();
-        {
-            const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
-            const int lane = int(threadIdx.x) & ((1 << log) - 1), rows = p1 - p0, full = rows / pc.rp;
-            for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
-                const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
-                const bool mine = gi < gn;
-                const int ca = max(c0, g * Cg), before = ca - g * Cg;   // channels of the group in earlier tiles
-                const int wd = (min(c1, (g + 1) * Cg) - ca) / (VEC / W), at = (ca - c0) / (VEC / W);
-                const float2 old = mine ? acc[g] : make_float2(0.0f, 0.0f);
-                const float about = mine ? part[at].x : 0.0f;   // row 0 is there if any is
-                Merge m;
-                if (mine) {
-                    for (int i = lane; i < pc.rp * wd; i += 1 << log) {
-                        const int r = wd == 1 ? i : i / wd;
-                        const float2 v = part[r * pc.nv * W + at + i - r * wd];
-                        const int cnt = full + (r < rows - full * pc.rp ? 1 : 0);
-                        m.add(about, float(cnt * (VEC / W)), v.x, v.y);
-                    }
-                    if (before > 0 && lane == 0) m.add(about, float(rows) * float(before), old.x, old.y);
-                }
-                m.lanes(log);
-                __syncwarp();
-                if (mine && lane == 0) acc[g] = m.pair(about, float(rows) * float(min(c1, (g + 1) * Cg) - g * Cg));
-            }
-        }
+        tile_moments<VEC, W>(pc, tile, Cg, p1 - p0, part, acc);
         __syncthreads();
     }
     for (int g = threadIdx.x; g < G; g += kGnThreads)
@@ -576,78 +690,28 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_moments_kernel(GnPlan pl) {
 }
 
 // Forward, sweep 2: merges the sample's chunks, writes y.
-template <typename T, int VEC, int ACT, bool ONEG, bool RING>
+template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ __align__(16) float gn_smem[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
-    float2* st = reinterpret_cast<float2*>(smem + (RING ? Ring<1>::bytes() : 0));   // [G] mean, rstd
-    constexpr int U = RING ? 4 : 8;
-    const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
+    extern __shared__ float gn_smem[];
+    float2* st = reinterpret_cast<float2*>(gn_smem);   // [G] mean, rstd
+    constexpr int U = 8;
+    const int C = int(a.C), Cg = C / int(a.G), cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
-    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     pdl_launch_dependents();
-    Ring<1> ring;
-    if constexpr (RING) {   // x is on its way while the partials are merged
-        const Place pc(cv, 0);
-        ring.init(smem, pv - p0, pc.rp * U, C * int(sizeof(T)), true);
-        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
-        ring.setup();
-        __syncthreads();
-        ring.fill();
-    }
     pdl_wait();
-    {
-        __shared__ Merge merged[kGnWarps][32];
-        const int parts = pl.chunks;
-        for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the partials
-            Merge m;
-            const float2* from = pl.moments + int64_t(n) * parts * G + g;
-            const float about = g < G ? from[0].x : 0.0f;
-            if (g < G)
-#pragma unroll 8
-                for (int k = warp; k < parts; k += kGnWarps) {
-                    const float2 v = from[int64_t(k) * G];
-                    m.add(about, float(rows_of(len, k, pl.rows)) * float(Cg), v.x, v.y);
-                }
-            merged[warp][lane] = m;
-            __syncthreads();
-            if (warp == 0 && g < G) {
-#pragma unroll
-                for (int k = 1; k < kGnWarps; ++k) {
-                    m.nd += merged[k][lane].nd;
-                    m.m2 += merged[k][lane].m2;
-                }
-                st[g] = mean_rstd(group_pivot(x, len, g * Cg), m.pair(about, float(len) * float(Cg)), len, Cg, a.eps);
-                if (chunk == 0) reinterpret_cast<float2*>(a.stats)[int64_t(n) * G + g] = st[g];
-            }
-            __syncthreads();
-        }
-    }
+    sample_stats(pl, n, chunk == 0, len, x, st);
+    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        if (!RING && !pc.on) continue;
+        if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
         Forward<T, VEC, ACT, ONEG> fw;
-        if (pc.on) fw.load(a, c, c, Cg, st);
-        for (int p = pv + pc.r; pc.on && p < pe; p += pc.rp)   // padding
-            store_pack<T, VEC>(y + int64_t(p) * C + c, pack_zero<T, VEC>());
-        if constexpr (RING) {
-            ring.run([&](const unsigned char* sx, int first, int rows) {
-                if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
-                const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + pc.v * VEC;
-                T* to = y + int64_t(p0 + first + pc.r) * C + c;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (pc.on && pc.r + u * pc.rp < rows)
-                        store_pack<T, VEC>(to + u * pc.rp * C, fw(load_pack<T, VEC>(at + u * pc.rp * C), a.act));
-            });
-            return;
-        }
+        fw.load(a, c, c, Cg, st);
+        pad_rows<T, VEC>(pc, y, C, c, pv, pe);
         int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
         const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
         T* yc = y + int64_t(pv - 1 - pc.r) * C + c;
@@ -664,201 +728,82 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
 }
 
 // Backward, sweep 1: per-channel and per-group sums over a chunk.
-template <typename T, int VEC, int ACT, bool ONEG, bool RING>
+template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_sums_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ __align__(16) float gn_smem[];
-    constexpr int U = RING ? 2 : 4;
+    extern __shared__ float gn_smem[];
+    constexpr int U = 4, NP = pairs_of(VEC);
     const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
-    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
-    float2* acc = reinterpret_cast<float2*>(smem + (RING ? Ring<2>::bytes() : 0));   // [G]
-    float2* part = RING ? reinterpret_cast<float2*>(smem) : acc + G;                 // [rp][nv * VEC], on the ring when it is done
+    float2* acc = reinterpret_cast<float2*>(gn_smem);   // [G]
+    float2* part = acc + G;                             // [rp][nv * VEC]
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int64_t slot = int64_t(n) * pl.chunks + chunk;
     const int len = valid_len(a, n);
     const int p0 = min(len, chunk * pl.rows), p1 = min(len, p0 + pl.rows);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
-    const float2* st = reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G;
     pdl_launch_dependents();
     for (int g = threadIdx.x; g < G; g += kGnThreads) acc[g] = make_float2(0.0f, 0.0f);
-    Ring<2> ring;
-    if constexpr (RING) {
-        const Place pc(cv, 0);
-        ring.init(smem, p1 - p0, pc.rp * U, C * int(sizeof(T)), false);
-        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
-        ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
-        ring.setup();
-    }
     __syncthreads();
-    if constexpr (RING) ring.fill();
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        const int c0 = tile * kGnThreads * VEC, c1 = c0 + pc.nv * VEC;
-        {
-            const int c = c0 + pc.v * VEC;
+        if (pc.on) {
+            const int c = (tile * kGnThreads + pc.v) * VEC;
             Backward<T, VEC, ACT, ONEG> bw;
-            if (pc.on) bw.load(a, c, c, Cg, st);
-            constexpr int NP = pairs_of(VEC);
+            bw.load(a, c, c, Cg, reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G);
             float2 sa[NP], sb[NP];
 #pragma unroll
             for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
-            if constexpr (RING) {
-                ring.run([&](const unsigned char* s0, int, int rows) {
-                    const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + pc.v * VEC;
-                    const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + pc.v * VEC;
+            int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
+            const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
+            const T* gc = dy + int64_t(p0 + pc.r) * a.gp + c;
+            const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp;
+            for (; left >= U; left -= U) {
+                Pack<T, VEC> rx[U], rg[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (pc.on && pc.r + u * pc.rp < rows)
-                            bw.sums(load_pack<T, VEC>(sx + u * pc.rp * C), load_pack<T, VEC>(sg + u * pc.rp * C), a.act,
-                                    sa, sb);
-                });
-                if (ring.dead) sa[0] = splat2(__int_as_float(0x7fffffff));
-                __syncthreads();   // the ring's memory is the partials' from here on
-            } else if (pc.on) {
-                int left = max(0, p1 - p0 - pc.r + pc.rp - 1) / pc.rp;
-                const T* xc = x + int64_t(p0 + pc.r) * a.xp + c;
-                const T* gc = dy + int64_t(p0 + pc.r) * a.gp + c;
-                const int64_t xs = int64_t(pc.rp) * a.xp, gs = int64_t(pc.rp) * a.gp;
-                for (; left >= U; left -= U) {
-                    Pack<T, VEC> rx[U], rg[U];
-#pragma unroll
-                    for (int u = 0; u < U; ++u, xc += xs, gc += gs) {
-                        rx[u] = load_pack<T, VEC>(xc);
-                        rg[u] = load_pack<T, VEC>(gc);
-                    }
-#pragma unroll
-                    for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
+                for (int u = 0; u < U; ++u, xc += xs, gc += gs) {
+                    rx[u] = load_pack<T, VEC>(xc);
+                    rg[u] = load_pack<T, VEC>(gc);
                 }
-                for (; left > 0; --left, xc += xs, gc += gs)
-                    bw.sums(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act, sa, sb);
-            }
-            if (pc.on)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                part[(pc.r * pc.nv + pc.v) * VEC + j] =
-                    j % 2 ? make_float2(sa[j / 2].y, sb[j / 2].y) : make_float2(sa[j / 2].x, sb[j / 2].x);
+                for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
+            }
+            for (; left > 0; --left, xc += xs, gc += gs)
+                bw.sums(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act, sa, sb);
+            put_pairs<VEC>(part + (pc.r * pc.nv + pc.v) * VEC, sa, sb);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < pc.nv * VEC; i += kGnThreads) {   // rows of a channel, in order
-            float2 s = part[i];
-            for (int r = 1; r < pc.rp; ++r) {
-                const float2 v = part[r * pc.nv * VEC + i];
-                s.x += v.x;
-                s.y += v.y;
-            }
-            part[i] = s;
-            pl.csums[slot * C + c0 + i] = s;
-        }
-        __syncthreads();
-        {
-            const int g0 = c0 / Cg, gn = (c1 - 1) / Cg - g0 + 1, log = lanes_log(gn, kGnThreads);
-            const int lane = int(threadIdx.x) & ((1 << log) - 1);
-            for (int i0 = 0; i0 < gn; i0 += kGnThreads >> log) {
-                const int gi = i0 + (int(threadIdx.x) >> log), g = g0 + gi;
-                float2 s = make_float2(0.0f, 0.0f);
-                if (gi < gn)
-                    for (int c = max(c0, g * Cg) + lane; c < min(c1, (g + 1) * Cg); c += 1 << log) {
-                        const float w = a.weight ? load_param(a.weight, a.param_dtype, c) : 1.0f;
-                        s.x += w * part[c - c0].x;
-                        s.y += w * part[c - c0].y;
-                    }
-                s = lanes_sum(s, log);
-                if (gi < gn && lane == 0) {
-                    acc[g].x += s.x;
-                    acc[g].y += s.y;
-                }
-            }
-        }
+        tile_sums<VEC>(pl, pc, tile, slot, part, acc);
         __syncthreads();
     }
     for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
 }
 
 // Backward, sweep 2: merges the sample's group sums, writes dx.
-template <typename T, int VEC, int ACT, bool ONEG, bool RING>
+template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
-    extern __shared__ __align__(16) float gn_smem[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>(gn_smem);
-    float4* gv = reinterpret_cast<float4*>(smem + (RING ? Ring<2>::bytes() : 0));   // [G] mean, rstd, S1/m, S2/m
-    constexpr int U = RING ? 2 : 4;
-    const int C = int(a.C), G = int(a.G), Cg = C / G, cv = C / VEC;
+    extern __shared__ float gn_smem[];
+    float4* gv = reinterpret_cast<float4*>(gn_smem);   // [G] mean, rstd, S1/m, S2/m
+    constexpr int U = 4;
+    const int C = int(a.C), Cg = C / int(a.G), cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float inv = len > 0 ? 1.0f / (float(len) * float(Cg)) : 0.0f;
+    pdl_launch_dependents();
+    pdl_wait();
+    sample_sums(pl, n, len, gv);
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
-    pdl_launch_dependents();
-    Ring<2> ring;
-    if constexpr (RING) {   // x and dy are on their way while the partials are merged
-        const Place pc(cv, 0);
-        ring.init(smem, pv - p0, pc.rp * U, C * int(sizeof(T)), true);
-        ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
-        ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
-        ring.setup();
-        __syncthreads();
-        ring.fill();
-    }
-    pdl_wait();
-    if (a.dweight || a.dbias) {   // the blocks share out the channels while their first rows arrive
-        const int per = (C + int(gridDim.x) - 1) / int(gridDim.x);
-        param_grads(pl, int(blockIdx.x) * per, min(C, int(blockIdx.x + 1) * per));
-    }
-    {
-        __shared__ float2 merged[kGnWarps][32];
-        const int parts = pl.chunks;
-        for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the partials
-            float2 s = make_float2(0.0f, 0.0f);
-            if (g < G)
-#pragma unroll 8
-                for (int k = warp; k < parts; k += kGnWarps) {
-                    const float2 v = pl.gsums[(int64_t(n) * parts + k) * G + g];
-                    s.x += v.x;
-                    s.y += v.y;
-                }
-            merged[warp][lane] = s;
-            __syncthreads();
-            if (warp == 0 && g < G) {
-#pragma unroll
-                for (int k = 1; k < kGnWarps; ++k) {
-                    s.x += merged[k][lane].x;
-                    s.y += merged[k][lane].y;
-                }
-                const float2 v = reinterpret_cast<const float2*>(a.stats)[int64_t(n) * G + g];
-                gv[g] = make_float4(v.x, v.y, s.x * inv, s.y * inv);
-            }
-            __syncthreads();
-        }
-    }
     T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
         const Place pc(cv, tile);
-        if (!RING && !pc.on) continue;
+        if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
         BackwardDx<T, VEC, ACT, ONEG> bw;
-        if (pc.on) {
-            bw.load(a, c, c, Cg, gv);
-            bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
-        }
-        for (int p = pv + pc.r; pc.on && p < pe; p += pc.rp)   // padding
-            store_pack<T, VEC>(dx + int64_t(p) * C + c, pack_zero<T, VEC>());
-        if constexpr (RING) {
-            ring.run([&](const unsigned char* s0, int first, int rows) {
-                if (ring.dead) bw.rw[0] = splat2(__int_as_float(0x7fffffff));
-                const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + pc.v * VEC;
-                const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + pc.v * VEC;
-                T* to = dx + int64_t(p0 + first + pc.r) * C + c;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (pc.on && pc.r + u * pc.rp < rows)
-                        store_pack<T, VEC>(to + u * pc.rp * C, bw.dx(load_pack<T, VEC>(sx + u * pc.rp * C),
-                                                                     load_pack<T, VEC>(sg + u * pc.rp * C), a.act));
-            });
-            return;
-        }
+        bw.load(a, c, c, Cg, gv);
+        bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
+        pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
         int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
         const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
         const T* gc = dy + int64_t(pv - 1 - pc.r) * a.gp + c;
@@ -877,6 +822,147 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
         for (; left > 0; --left, xc -= xs, gc -= gs, dc -= ds)
             store_pack<T, VEC>(dc, bw.dx(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act));
     }
+}
+
+// ---- both sweeps in one launch --------------------------------------------------
+//
+// For rows one after another in memory: the same two sweeps on the ring, with a
+// grid barrier between them where a sample's chunks lie in several blocks (a
+// cooperative launch, one block per SM), so the second one finds the last 160 KB
+// of every block's rows on chip and no launch lies between them.
+
+template <typename T, int VEC, int ACT, bool ONEG>
+__global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) {
+    const GroupNormArgs& a = pl.a;
+    extern __shared__ __align__(16) unsigned char gn_ring[];
+    constexpr int W = ONEG ? 1 : VEC, U = 4;
+    const int C = int(a.C), G = int(a.G), Cg = C / G;
+    float2* acc = reinterpret_cast<float2*>(gn_ring + Ring<1>::bytes());   // [G] mean, M; then mean, rstd
+    float2* part = acc + (G + 1) / 2 * 2;                                  // [rp][nv * W]
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int len = valid_len(a, n);
+    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
+    const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
+    const Place pc(C / VEC, 0);
+    const int c = pc.v * VEC;
+    Ring<1> ring;
+    ring.init(gn_ring, max(pv - p0, 0), pc.rp * U, C * int(sizeof(T)));
+    ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+    __syncthreads();
+    ring.fill();
+    {
+        PerGroup<VEC, ONEG> pivot;
+        if (pc.on) pivot.fill(c, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
+        Running<T, VEC, ONEG> run;
+        Batch<T, VEC, ONEG> bt;
+        ring.forwards([&](const unsigned char* sx, int, int rows) {
+            const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + c;
+            const int k = pc.on ? (rows - pc.r + pc.rp - 1) / pc.rp : 0;
+            Pack<T, VEC> raw[U];
+            if (k == U) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                bt.template take<U, true>(raw, pivot, U);
+                run.join(bt, float(U));
+            } else if (k > 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u < k) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                bt.template take<U, false>(raw, pivot, k);
+                run.join(bt, float(k));
+            }
+        });
+        if (ring.dead) run.mean[0] = __int_as_float(0x7fffffff);
+        if (pc.on)
+#pragma unroll
+            for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(run.mean[j], run.m2[j]);
+    }
+    __syncthreads();
+    tile_moments<VEC, W>(pc, 0, Cg, max(pv - p0, 0), part, acc);
+    __syncthreads();
+    for (int g = threadIdx.x; g < G; g += kGnThreads)
+        pl.moments[(int64_t(n) * pl.chunks + chunk) * G + g] = acc[g];
+    if (pl.chunks > 1)
+        cooperative_groups::this_grid().sync();
+    else
+        __syncthreads();
+    sample_stats(pl, n, chunk == 0, len, x, acc);
+    T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
+    Forward<T, VEC, ACT, ONEG> fw;
+    if (pc.on) fw.load(a, c, c, Cg, acc);
+    ring.backwards([&](const unsigned char* sx, int first, int rows) {
+        if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
+        const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + c;
+        T* to = y + int64_t(p0 + first + pc.r) * C + c;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (pc.on && pc.r + u * pc.rp < rows)
+                store_pack<T, VEC>(to + u * pc.rp * C, fw(load_pack<T, VEC>(at + u * pc.rp * C), a.act));
+    });
+    pad_rows<T, VEC>(pc, y, C, c, pv, pe);
+}
+
+template <typename T, int VEC, int ACT, bool ONEG>
+__global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) {
+    const GroupNormArgs& a = pl.a;
+    extern __shared__ __align__(16) unsigned char gn_ring[];
+    constexpr int U = 2, NP = pairs_of(VEC);
+    const int C = int(a.C), G = int(a.G), Cg = C / G;
+    float4* gv = reinterpret_cast<float4*>(gn_ring + Ring<2>::bytes());   // [G] mean, rstd, S1/m, S2/m
+    float2* acc = reinterpret_cast<float2*>(gv + G);                      // [G]
+    float2* part = acc + (G + 1) / 2 * 2;                                 // [rp][nv * VEC]
+    const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
+    const int64_t slot = int64_t(n) * pl.chunks + chunk;
+    const int len = valid_len(a, n);
+    const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
+    const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
+    const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
+    const Place pc(C / VEC, 0);
+    const int c = pc.v * VEC;
+    Ring<2> ring;
+    ring.init(gn_ring, max(pv - p0, 0), pc.rp * U, C * int(sizeof(T)));
+    ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
+    ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
+    for (int g = threadIdx.x; g < G; g += kGnThreads) acc[g] = make_float2(0.0f, 0.0f);
+    __syncthreads();
+    ring.fill();
+    BackwardDx<T, VEC, ACT, ONEG> bw;
+    if (pc.on) bw.load(a, c, c, Cg, reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G);
+    {
+        float2 sa[NP], sb[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) sa[j] = sb[j] = splat2(0.0f);
+        ring.forwards([&](const unsigned char* s0, int, int rows) {
+            const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + c;
+            const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + c;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (pc.on && pc.r + u * pc.rp < rows)
+                    bw.sums(load_pack<T, VEC>(sx + u * pc.rp * C), load_pack<T, VEC>(sg + u * pc.rp * C), a.act, sa, sb);
+        });
+        if (ring.dead) sa[0] = splat2(__int_as_float(0x7fffffff));
+        if (pc.on) put_pairs<VEC>(part + (pc.r * pc.nv + pc.v) * VEC, sa, sb);
+    }
+    __syncthreads();
+    tile_sums<VEC>(pl, pc, 0, slot, part, acc);
+    __syncthreads();
+    for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
+    cooperative_groups::this_grid().sync();   // the parameters' gradients need every block's sums
+    sample_sums(pl, n, len, gv);
+    T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
+    if (pc.on) bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
+    ring.backwards([&](const unsigned char* s0, int first, int rows) {
+        if (ring.dead) bw.rw[0] = splat2(__int_as_float(0x7fffffff));
+        const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + c;
+        const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + c;
+        T* to = dx + int64_t(p0 + first + pc.r) * C + c;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (pc.on && pc.r + u * pc.rp < rows)
+                store_pack<T, VEC>(to + u * pc.rp * C, bw.dx(load_pack<T, VEC>(sx + u * pc.rp * C),
+                                                             load_pack<T, VEC>(sg + u * pc.rp * C), a.act));
+    });
+    pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
 }
 
 // ---- resident path ------------------------------------------------------------
@@ -1134,8 +1220,24 @@ size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward
     return sweeps > resident ? sweeps : resident;
 }
 
+// How a launch stands to the one before it, or to its own blocks.
+enum LaunchKind { kPlain, kDependent, kCooperative };
+
+// Whether the device takes a cooperative launch of one block for each of kSMs SMs.
+bool cooperative_device() {
+    static int known[64] = {};   // 0: not asked yet, 1: yes, -1: no
+    int dev = 0, sms = 0, coop = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (known[dev] == 0) {
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        cudaDeviceGetAttribute(&coop, cudaDevAttrCooperativeLaunch, dev);
+        known[dev] = sms >= kSMs && coop ? 1 : -1;
+    }
+    return known[dev] > 0;
+}
+
 template <typename K>
-int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem, int cluster, bool dependent,
+int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem, int cluster, LaunchKind kind,
            cudaStream_t st) {
     if (blocks > 0x7fffffff) return fail(DOT_ERR_UNSUPPORTED, "group norm: too many blocks");
     if (smem > 48 * 1024) {
@@ -1156,9 +1258,14 @@ int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem,
         attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
         ++n;
     }
-    if (dependent) {
+    if (kind == kDependent) {
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    if (kind == kCooperative) {
+        attr[n].id = cudaLaunchAttributeCooperative;
+        attr[n].val.cooperative = 1;
         ++n;
     }
     cfg.attrs = attr;
@@ -1170,7 +1277,7 @@ int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem,
 int launch_params(const GnPlan& pl, cudaStream_t st) {
     if (!pl.a.dweight && !pl.a.dbias) return DOT_OK;
     ProfScope ps(DOT_K_NORM_BWD, st);
-    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, kGnWarps), kGnThreads, 0, 1, true, st);
+    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, kGnWarps), kGnThreads, 0, 1, kDependent, st);
 }
 
 // The resident plan of a problem, if its blocks hold it in registers all at
@@ -1211,46 +1318,61 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
     const int64_t blocks = pl.a.N * pl.slabs * pl.chunks;
     if (!backward) {
         ProfScope ps(DOT_K_NORM_FWD, st);
-        return launch(gn_resident_fwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, false, st);
+        return launch(gn_resident_fwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, kPlain, st);
     }
     int rc = DOT_OK;
     if constexpr (KV <= res_vecs(VEC * sizeof(T), true)) {
         carve(ws, pl, true);
         ProfScope ps(DOT_K_NORM_BWD, st);
-        rc = launch(gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, false, st);
+        rc = launch(gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, kPlain, st);
     }
     return rc ? rc : launch_params(pl, st);
 }
 
-template <typename T, int VEC, int ACT, bool ONEG, bool RING>
+template <typename T, int VEC, int ACT, bool ONEG>
 int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     const GroupNormArgs& a = pl.a;
     sweep_plan(pl);
     carve(ws, pl, backward);
-    const size_t base = RING ? (backward ? Ring<2>::bytes() : Ring<1>::bytes()) : 0;
-    const size_t part = RING ? 0 : size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
-    const size_t s1 = base + (size_t(a.G) + part) * sizeof(float2);
-    const size_t s2 = base + size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
+    const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
+    const size_t s1 = (size_t(a.G) + part) * sizeof(float2);
+    const size_t s2 = size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
     const int64_t blocks = a.N * pl.chunks;
     const bool second = !backward || a.dx != nullptr;
     int rc;
     {
         ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st, second ? 2 : 1);
-        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s1, 1, false, st)
-                      : launch(gn_moments_kernel<T, VEC, ONEG, RING>, pl, blocks, kGnThreads, s1, 1, false, st);
+        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, kPlain, st)
+                      : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, kPlain, st);
         if (!rc && second)
-            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s2, 1, true, st)
-                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG, RING>, pl, blocks, kGnThreads, s2, 1, true, st);
+            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, kDependent, st)
+                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, kDependent, st);
     }
     if (rc) return rc;
     return backward && !second ? launch_params(pl, st) : DOT_OK;
 }
 
-// Whether the sweeps take their rows by bulk copies: rows one after another in
-// memory, of whole 16-byte vectors, at most one per thread, and groups few
-// enough to leave the ring its shared memory.
-bool ring_rows(const GroupNormArgs& a, int vec, bool backward) {
-    return a.C / vec <= kGnThreads && a.G <= 1024 && a.xp == a.C && (!backward || a.gp == a.C);
+// Both sweeps in one launch, where the rows lie one after another in memory, a
+// row's vectors are at most one per thread, the groups leave the ring its shared
+// memory, and every block that waits for others has an SM of its own.
+template <typename T, int VEC, int ACT, bool ONEG>
+bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
+    const GroupNormArgs& a = pl.a;
+    if (a.C / VEC > kGnThreads || a.G > 1024 || a.xp != a.C || (backward && (a.gp != a.C || a.dx == nullptr)))
+        return false;
+    sweep_plan(pl);
+    const int64_t blocks = a.N * pl.chunks;
+    const bool waits = backward || pl.chunks > 1;
+    if (waits && (blocks > kSMs || !cooperative_device())) return false;
+    carve(ws, pl, backward);
+    const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1) * sizeof(float2);
+    const size_t groups = size_t(a.G + 1) * (backward ? sizeof(float4) + sizeof(float2) : sizeof(float2));
+    ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st);
+    rc = backward ? launch(gn_fused_bwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
+                           Ring<2>::bytes() + groups + part, 1, kCooperative, st)
+                  : launch(gn_fused_fwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
+                           Ring<1>::bytes() + groups + part, 1, waits ? kCooperative : kPlain, st);
+    return true;
 }
 
 template <typename T, int VEC, int ACT, bool ONEG>
@@ -1259,9 +1381,11 @@ int run(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st) {
     pl.a = a;
     int threads, vecs;
     if (!resident_plan(pl, VEC, sizeof(T), backward, threads, vecs)) {
-        if constexpr (VEC * sizeof(T) == 16)
-            if (ring_rows(a, VEC, backward)) return sweep_run<T, VEC, ACT, ONEG, true>(pl, ws, backward, st);
-        return sweep_run<T, VEC, ACT, ONEG, false>(pl, ws, backward, st);
+        if constexpr (VEC * sizeof(T) == 16) {
+            int rc = DOT_OK;
+            if (fused_run<T, VEC, ACT, ONEG>(pl, ws, backward, st, rc)) return rc;
+        }
+        return sweep_run<T, VEC, ACT, ONEG>(pl, ws, backward, st);
     }
     constexpr int most = res_vecs(VEC * sizeof(T), true);
     if (vecs <= most / 4) return resident_run<T, VEC, ACT, ONEG, most / 4>(pl, ws, threads, backward, st);

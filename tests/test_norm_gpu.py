@@ -455,3 +455,68 @@ def test_a_recorded_backward_is_not_differentiated_again():
     (g,) = torch.autograd.grad(dot.group_norm_act(x, 4).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once differentiable"):
         (g.sum() + x.sum()).backward()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,S,C,G,lengths", [
+    (2, 40000, 64, 8, None),               # a vector in one group
+    (1, 60001, 48, 24, None),              # groups across vectors, an odd end
+    (3, 30011, 64, 4, [30011, 0, 17]),     # empty and nearly empty chunks
+    (5, 17000, 40, 5, [1, 16999, 4096, 0, 8000]),
+    (200, 65, 128, 32, None),              # more samples than SMs
+    (149, 1, 512, 2, None),
+    (1, 9000, 1024, 8, None),
+    (160, 40, 24, 3, [40 - (7 * n) % 41 for n in range(160)]),
+])
+def test_beyond_one_cluster(N, S, C, G, lengths, dtype, strided):
+    """Sizes that no cluster's registers hold, rows one after another and rows cut from wider ones."""
+    x, dy, w, b = inputs(N, S, C, dtype, torch.float32, N + S)
+    if strided:
+        x, dy = strided_rows(x), strided_rows(dy)
+    y, grads = check(x, dy, G, w, b, "silu", lengths)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    again = dot.group_norm_act(leaves[0], G, leaves[1], leaves[2], lengths=ln)
+    assert torch.equal(again, y)
+    for got, want in zip(torch.autograd.grad(again, leaves, dy), grads):
+        assert torch.equal(got, want)
+
+
+def strided_rows(x):
+    wide = torch.full((*x.shape[:2], x.size(2) + 16), 7.0, device=DEV, dtype=x.dtype)
+    wide[..., 8:8 + x.size(2)] = x
+    return wide[..., 8:8 + x.size(2)]
+
+
+def test_a_large_call_in_a_graph():
+    x, dy, w, b = inputs(2, 30000, 64, torch.bfloat16, torch.float32, 15)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    torch.autograd.grad(dot.group_norm_act(leaves[0], 8, leaves[1], leaves[2]), leaves, dy)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dot.group_norm_act(leaves[0], 8, leaves[1], leaves[2])
+        grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        x.mul_(1.5).add_(0.25)
+    for _ in range(2):
+        graph.replay()
+    want = dot.group_norm_act(leaves[0], 8, leaves[1], leaves[2])
+    assert torch.equal(y, want)
+    for got, ref in zip(grads, torch.autograd.grad(want, leaves, dy)):
+        assert torch.equal(got, ref)
+
+
+def test_large_calls_on_two_streams():
+    """Calls whose blocks wait for one another, at the same time on two streams."""
+    x, dy, w, b = inputs(2, 30000, 64, torch.bfloat16, torch.float32, 16)
+    want = dot.group_norm_act(x, 8, w, b)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for s, o in zip(streams, outs):
+            with torch.cuda.stream(s):
+                o.append(dot.group_norm_act(x, 8, w, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for o in outs for t in o)
