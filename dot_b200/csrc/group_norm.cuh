@@ -165,8 +165,14 @@ struct Forward {
     float2 scale[NP], shift[NP];
     // st: (mean, rstd) by group; c: the first channel, c_st: counted from st's first group
     __device__ __forceinline__ void load(const GroupNormArgs& a, int c, int c_st, int Cg, const float2* st) {
+        params(a, c);
+        stats(c_st, Cg, st);
+    }
+    __device__ __forceinline__ void params(const GroupNormArgs& a, int c) {
         load_params<VEC>(a.weight, a.param_dtype, c, 1.0f, scale);
         load_params<VEC>(a.bias, a.param_dtype, c, 0.0f, shift);
+    }
+    __device__ __forceinline__ void stats(int c_st, int Cg, const float2* st) {
         mean.fill(c_st, Cg, [&](int g) { return st[g].x; });
         PerGroup<VEC, ONEG> r;
         r.fill(c_st, Cg, [&](int g) { return st[g].y; });
@@ -274,6 +280,12 @@ __device__ __forceinline__ void param_grads(const GnPlan& pl, int first, int end
             if (a.dweight) store_param(a.dweight, a.param_dtype, c, s.y);
         }
     }
+}
+
+// The blocks of a launch share out the channels.
+__device__ __forceinline__ void share_param_grads(const GnPlan& pl) {
+    const int C = int(pl.a.C), per = (C + int(gridDim.x) - 1) / int(gridDim.x);
+    if (pl.a.dweight || pl.a.dbias) param_grads(pl, int(blockIdx.x) * per, min(C, int(blockIdx.x + 1) * per));
 }
 
 // A launch of its own where no other one follows the sums.
@@ -523,9 +535,10 @@ __device__ __forceinline__ void tile_moments(const Place& pc, int tile, int Cg, 
     }
 }
 
-// Statistics [G] of sample n from its chunks' moments, by the whole block.
-template <typename T>
-__device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write, int len, const T* x, float2* st) {
+// Statistics [G] of sample n from its chunks' moments, by the whole block;
+// pivot(g): the value that group g's moments are about.
+template <typename F>
+__device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write, int len, F pivot, float2* st) {
     __shared__ Merge merged[kGnWarps][32];
     const GroupNormArgs& a = pl.a;
     const int G = int(a.G), Cg = int(a.C) / G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -547,7 +560,7 @@ __device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write
                 m.nd += merged[k][lane].nd;
                 m.m2 += merged[k][lane].m2;
             }
-            st[g] = mean_rstd(group_pivot(x, len, g * Cg), m.pair(about, float(len) * float(Cg)), len, Cg, a.eps);
+            st[g] = mean_rstd(pivot(g), m.pair(about, float(len) * float(Cg)), len, Cg, a.eps);
             if (write) reinterpret_cast<float2*>(a.stats)[int64_t(n) * G + g] = st[g];
         }
         __syncthreads();
@@ -591,16 +604,13 @@ __device__ __forceinline__ void tile_sums(const GnPlan& pl, const Place& pc, int
 }
 
 // Mean, rstd, S1/m and S2/m [G] of sample n from its chunks' sums, by the whole
-// block; the blocks of the launch share out the parameters' gradients.
-__device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, float4* gv) {
+// block; stats(g): mean and rstd of group g.
+template <typename F>
+__device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, F stats, float4* gv) {
     __shared__ float2 merged[kGnWarps][32];
     const GroupNormArgs& a = pl.a;
     const int C = int(a.C), G = int(a.G), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv = len > 0 ? 1.0f / (float(len) * float(C / G)) : 0.0f;
-    if (a.dweight || a.dbias) {
-        const int per = (C + int(gridDim.x) - 1) / int(gridDim.x);
-        param_grads(pl, int(blockIdx.x) * per, min(C, int(blockIdx.x + 1) * per));
-    }
     for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the chunks
         float2 s = make_float2(0.0f, 0.0f);
         if (g < G)
@@ -618,7 +628,7 @@ __device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, fl
                 s.x += merged[k][lane].x;
                 s.y += merged[k][lane].y;
             }
-            const float2 v = reinterpret_cast<const float2*>(a.stats)[int64_t(n) * G + g];
+            const float2 v = stats(g);
             gv[g] = make_float4(v.x, v.y, s.x * inv, s.y * inv);
         }
         __syncthreads();
@@ -702,7 +712,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_apply_kernel(GnPlan pl) {
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     pdl_launch_dependents();
     pdl_wait();
-    sample_stats(pl, n, chunk == 0, len, x, st);
+    sample_stats(pl, n, chunk == 0, len, [&](int g) { return group_pivot(x, len, g * Cg); }, st);
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
     for (int tile = 0; tile * kGnThreads < cv; ++tile) {
@@ -791,7 +801,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const int len = valid_len(a, n);
     pdl_launch_dependents();
     pdl_wait();
-    sample_sums(pl, n, len, gv);
+    sample_sums(pl, n, len, [&](int g) { return reinterpret_cast<const float2*>(a.stats)[int64_t(n) * a.G + g]; }, gv);
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
@@ -822,6 +832,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
         for (; left > 0; --left, xc -= xs, gc -= gs, dc -= ds)
             store_pack<T, VEC>(dc, bw.dx(load_pack<T, VEC>(xc), load_pack<T, VEC>(gc), a.act));
     }
+    share_param_grads(pl);
 }
 
 // ---- both sweeps in one launch --------------------------------------------------
@@ -838,7 +849,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
     constexpr int W = ONEG ? 1 : VEC, U = 4;
     const int C = int(a.C), G = int(a.G), Cg = C / G;
     float2* acc = reinterpret_cast<float2*>(gn_ring + Ring<1>::bytes());   // [G] mean, M; then mean, rstd
-    float2* part = acc + (G + 1) / 2 * 2;                                  // [rp][nv * W]
+    float* piv = reinterpret_cast<float*>(acc + G);                        // [G]
+    float2* part = acc + (G + 1) / 2 * 3;                                  // [rp][nv * W]
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
@@ -850,9 +862,11 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
     ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
     __syncthreads();
     ring.fill();
+    for (int g = threadIdx.x; g < G; g += kGnThreads) piv[g] = group_pivot(x, len, g * Cg);
+    __syncthreads();
     {
         PerGroup<VEC, ONEG> pivot;
-        if (pc.on) pivot.fill(c, Cg, [&](int g) { return group_pivot(x, len, g * Cg); });
+        if (pc.on) pivot.fill(c, Cg, [&](int g) { return piv[g]; });
         Running<T, VEC, ONEG> run;
         Batch<T, VEC, ONEG> bt;
         ring.forwards([&](const unsigned char* sx, int, int rows) {
@@ -882,14 +896,15 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
     __syncthreads();
     for (int g = threadIdx.x; g < G; g += kGnThreads)
         pl.moments[(int64_t(n) * pl.chunks + chunk) * G + g] = acc[g];
+    Forward<T, VEC, ACT, ONEG> fw;
+    if (pc.on) fw.params(a, c);   // on their way over the barrier
     if (pl.chunks > 1)
         cooperative_groups::this_grid().sync();
     else
         __syncthreads();
-    sample_stats(pl, n, chunk == 0, len, x, acc);
+    sample_stats(pl, n, chunk == 0, len, [&](int g) { return piv[g]; }, acc);
     T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
-    Forward<T, VEC, ACT, ONEG> fw;
-    if (pc.on) fw.load(a, c, c, Cg, acc);
+    if (pc.on) fw.stats(c, Cg, acc);
     ring.backwards([&](const unsigned char* sx, int first, int rows) {
         if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
         const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + c;
@@ -923,11 +938,16 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     ring.init(gn_ring, max(pv - p0, 0), pc.rp * U, C * int(sizeof(T)));
     ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
     ring.src[1] = reinterpret_cast<const unsigned char*>(dy + int64_t(p0) * C);
-    for (int g = threadIdx.x; g < G; g += kGnThreads) acc[g] = make_float2(0.0f, 0.0f);
     __syncthreads();
     ring.fill();
+    for (int g = threadIdx.x; g < G; g += kGnThreads) {
+        const float2 v = reinterpret_cast<const float2*>(a.stats)[int64_t(n) * G + g];
+        gv[g] = make_float4(v.x, v.y, 0.0f, 0.0f);
+        acc[g] = make_float2(0.0f, 0.0f);
+    }
+    __syncthreads();
     BackwardDx<T, VEC, ACT, ONEG> bw;
-    if (pc.on) bw.load(a, c, c, Cg, reinterpret_cast<const float2*>(a.stats) + int64_t(n) * G);
+    if (pc.on) bw.load(a, c, c, Cg, gv);
     {
         float2 sa[NP], sb[NP];
 #pragma unroll
@@ -948,7 +968,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     __syncthreads();
     for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
     cooperative_groups::this_grid().sync();   // the parameters' gradients need every block's sums
-    sample_sums(pl, n, len, gv);
+    sample_sums(pl, n, len, [&](int g) { return make_float2(gv[g].x, gv[g].y); }, gv);
     T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
     if (pc.on) bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
     ring.backwards([&](const unsigned char* s0, int first, int rows) {
@@ -963,6 +983,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
                                                              load_pack<T, VEC>(sg + u * pc.rp * C), a.act));
     });
     pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
+    share_param_grads(pl);
 }
 
 // ---- resident path ------------------------------------------------------------
@@ -1366,7 +1387,7 @@ bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
     if (waits && (blocks > kSMs || !cooperative_device())) return false;
     carve(ws, pl, backward);
     const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1) * sizeof(float2);
-    const size_t groups = size_t(a.G + 1) * (backward ? sizeof(float4) + sizeof(float2) : sizeof(float2));
+    const size_t groups = size_t(a.G + 1) * (backward ? sizeof(float4) + sizeof(float2) : sizeof(float2) + sizeof(float));
     ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st);
     rc = backward ? launch(gn_fused_bwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
                            Ring<2>::bytes() + groups + part, 1, kCooperative, st)
