@@ -19,8 +19,9 @@ int check_norm(int dtype, int param_dtype, int64_t N, int64_t S, int64_t C, int6
     if (!float_dtype(dtype) || !float_dtype(param_dtype))
         return fail(DOT_ERR_UNSUPPORTED, "dtype must be float32, bfloat16 or float16");
     if (activation < DOT_ACT_NONE || activation > DOT_ACT_RELU) return fail(DOT_ERR_INVALID, "unknown activation");
-    // positions and channels are 32-bit indices in the kernels, addresses 64-bit
-    if (S > 0x7fffffff || C > 0x7fffff || N > 0x7fffff) return fail(DOT_ERR_UNSUPPORTED, "dimension too large");
+    // positions and channels are 32-bit indices in the kernels (a thread's walk ends up
+    // to a block's rows past S), addresses 64-bit
+    if (S > 0x7fff0000 || C > 0x7fffff || N > 0x7fffff) return fail(DOT_ERR_UNSUPPORTED, "dimension too large");
     return DOT_OK;
 }
 

@@ -11,10 +11,15 @@
 // positions.  ONEG: a vector never crosses a group (VEC divides C/G), so its
 // statistics are one value each.
 //
-// Two paths, chosen by size (resident_plan): a cluster of blocks that holds its
-// share of a sample in registers and reads it once, and two sweeps for samples
-// beyond that.  No atomics; every merge has a fixed order, so results are
-// bitwise reproducible.
+// Three forms, chosen by size and layout (run): a cluster of blocks that holds
+// its share of a sample in registers and reads it once; beyond that, for rows
+// one after another in memory, one cooperative launch that walks them twice;
+// else the same two walks as two launches.  No atomics on values; every merge
+// has a fixed order, so results are bitwise reproducible.
+//
+// Measured (device time, 6.55 TB/s copy rate): 8 x 4800 x 256 bfloat16 with silu
+// 16.7 us forward; 16 x 76800 x 64 with relu 81.7 us; 2 x 76800 x 256 with silu
+// 46.9 us forward and 71.9 backward; 16 x 1024 x 256 padded sets 7.7 and 13.3.
 //
 // Moments are kept as (mean, sum M of squared deviations) of x - pivot, the
 // pivot one of the group's values: a mean far from zero then costs its own
@@ -37,7 +42,9 @@ namespace {
 
 constexpr int kSMs = 148;
 // One block of 512 threads per SM: up to 128 registers a thread, so that enough
-// loads are in flight (8 of 16 bytes a thread, 64 KB per SM).
+// loads are in flight (8 of 16 bytes a thread, 64 KB per SM).  1024 threads of
+// 64 registers measured 90 us where these take 84 (clip backward in two
+// launches); two blocks per SM are packed onto half the SMs.
 constexpr int kGnThreads = 512;
 constexpr int kGnWarps = kGnThreads / 32;
 constexpr int kMaxCluster = 8;
@@ -296,8 +303,9 @@ __global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
 
 // ---- two sweeps per direction --------------------------------------------------
 //
-// A block reads whole rows of one chunk (a range of one sample's positions).
-// The first sweep leaves the chunk's partial sums in the workspace, the second
+// For strided rows, vectors under 16 bytes and what the other forms do not
+// take.  A block reads whole rows of one chunk (a range of one sample's
+// positions).  The first sweep leaves the chunk's partial sums in the workspace, the second
 // merges its sample's partials at its start and writes the result, walking its
 // rows backwards: it begins with those that the first sweep read last.
 
@@ -840,7 +848,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
 // For rows one after another in memory: the same two sweeps on the ring, with a
 // grid barrier between them where a sample's chunks lie in several blocks (a
 // cooperative launch, one block per SM), so the second one finds the last 160 KB
-// of every block's rows on chip and no launch lies between them.
+// of every block's rows on chip and no launch lies between them.  Against two
+// launches with plain loads: 8 x 4800 x 256 18.9 -> 16.7 us, clip backward 90 ->
+// 72.  HBM bounds the way forwards, the SFU (two operations per element of
+// silu) or HBM the way back.
 
 template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) {
@@ -991,7 +1002,9 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
 // A cluster of `chunks` blocks holds one sample's positions of one channel slab
 // (whole groups) in registers: x (and dy) are read once, the blocks exchange
 // their groups' partial sums through distributed shared memory, and the result
-// is written from the registers.  One launch per direction.
+// is written from the registers.  One launch per direction (and a small one for
+// the parameters' gradients, which cross clusters).  Bound by latency: 3.4 us
+// for one 64 x 64 sample, 7.7 us forward and 13.3 us backward for 8.4 MB.
 
 // Where a block stands: chunk (its rank in the cluster), slab, sample.
 struct ResPlace {

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks<T>()) rotary_kernel(Ro
     const int64_t t0 = int64_t(blockIdx.x) * pl.tokens;
     const int nt = int(min(int64_t(pl.tokens), pl.ntok - t0));
     const int64_t b0 = pl.ntok <= 0x7fffffff ? int64_t(pl.by_len.div(int(t0))) : t0 / a.L;
-    const int l0 = int(t0 - b0 * a.L);   // and at most 256 tokens on: below 2^31
+    const int l0 = int(t0 - b0 * a.L);   // and at most 128 tokens on: below 2^31
 
     // A thread's work: token tl, `heads` consecutive heads of q or of k, and the
     // offsets o0, o1 of its two vectors within a head.
@@ -225,6 +225,7 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
     pl.q_runs = int(ceil_div(a.Hq, pl.run));
     pl.runs = pl.q_runs + int(ceil_div(a.Hk, pl.run));
     const int64_t per_token = int64_t(pl.slots) * pl.runs;
+    if (per_token > 0x3fffffff) return fail(DOT_ERR_UNSUPPORTED, "too many heads in a token");
     int64_t tokens = per_token >= kRotThreads ? 1 : kRotThreads / per_token;
     const int64_t fit = a.P > 0 ? kMaxPairs / a.P : tokens;
     if (tokens > fit) tokens = fit;
