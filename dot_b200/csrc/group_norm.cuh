@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const Place pc(C / VEC, 0);
-    const int c = pc.v * VEC;
+    const int c = pc.v * VEC, step = pc.rp * C;   // elements from a thread's row to its next
     Ring<1> ring;
     ring.init(gn_ring, max(pv - p0, 0), pc.rp * U, C * int(sizeof(T)));
     ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
@@ -886,13 +886,13 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
             Pack<T, VEC> raw[U];
             if (k == U) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * step);
                 bt.template take<U, true>(raw, pivot, U);
                 run.join(bt, float(U));
             } else if (k > 0) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (u < k) raw[u] = load_pack<T, VEC>(at + u * pc.rp * C);
+                    if (u < k) raw[u] = load_pack<T, VEC>(at + u * step);
                 bt.template take<U, false>(raw, pivot, k);
                 run.join(bt, float(k));
             }
@@ -920,10 +920,19 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
         if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
         const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + c;
         T* to = y + int64_t(p0 + first + pc.r) * C + c;
+        if (!pc.on) return;
+        if (rows == ring.stage_rows) {   // a whole stage: its vectors side by side
+            Pack<T, VEC> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (pc.on && pc.r + u * pc.rp < rows)
-                store_pack<T, VEC>(to + u * pc.rp * C, fw(load_pack<T, VEC>(at + u * pc.rp * C), a.act));
+            for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(at + u * step);
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = fw(raw[u], a.act);
+#pragma unroll
+            for (int u = 0; u < U; ++u) store_pack<T, VEC>(to + u * step, raw[u]);
+        } else {
+            for (int r = pc.r; r < rows; r += pc.rp, at += step, to += step)
+                store_pack<T, VEC>(to, fw(load_pack<T, VEC>(at), a.act));
+        }
     });
     pad_rows<T, VEC>(pc, y, C, c, pv, pe);
 }
@@ -944,7 +953,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
     const Place pc(C / VEC, 0);
-    const int c = pc.v * VEC;
+    const int c = pc.v * VEC, step = pc.rp * C;   // elements from a thread's row to its next
     Ring<2> ring;
     ring.init(gn_ring, max(pv - p0, 0), pc.rp * U, C * int(sizeof(T)));
     ring.src[0] = reinterpret_cast<const unsigned char*>(x + int64_t(p0) * C);
@@ -966,10 +975,20 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
         ring.forwards([&](const unsigned char* s0, int, int rows) {
             const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + c;
             const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + c;
+            if (!pc.on) return;
+            if (rows == ring.stage_rows) {   // a whole stage: its vectors side by side
+                Pack<T, VEC> rx[U], rg[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (pc.on && pc.r + u * pc.rp < rows)
-                    bw.sums(load_pack<T, VEC>(sx + u * pc.rp * C), load_pack<T, VEC>(sg + u * pc.rp * C), a.act, sa, sb);
+                for (int u = 0; u < U; ++u) {
+                    rx[u] = load_pack<T, VEC>(sx + u * step);
+                    rg[u] = load_pack<T, VEC>(sg + u * step);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) bw.sums(rx[u], rg[u], a.act, sa, sb);
+            } else {
+                for (int r = pc.r; r < rows; r += pc.rp, sx += step, sg += step)
+                    bw.sums(load_pack<T, VEC>(sx), load_pack<T, VEC>(sg), a.act, sa, sb);
+            }
         });
         if (ring.dead) sa[0] = splat2(__int_as_float(0x7fffffff));
         if (pc.on) put_pairs<VEC>(part + (pc.r * pc.nv + pc.v) * VEC, sa, sb);
@@ -987,11 +1006,22 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
         const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + c;
         const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + c;
         T* to = dx + int64_t(p0 + first + pc.r) * C + c;
+        if (!pc.on) return;
+        if (rows == ring.stage_rows) {   // a whole stage: its vectors side by side
+            Pack<T, VEC> rx[U], rg[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (pc.on && pc.r + u * pc.rp < rows)
-                store_pack<T, VEC>(to + u * pc.rp * C, bw.dx(load_pack<T, VEC>(sx + u * pc.rp * C),
-                                                             load_pack<T, VEC>(sg + u * pc.rp * C), a.act));
+            for (int u = 0; u < U; ++u) {
+                rx[u] = load_pack<T, VEC>(sx + u * step);
+                rg[u] = load_pack<T, VEC>(sg + u * step);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) rx[u] = bw.dx(rx[u], rg[u], a.act);
+#pragma unroll
+            for (int u = 0; u < U; ++u) store_pack<T, VEC>(to + u * step, rx[u]);
+        } else {
+            for (int r = pc.r; r < rows; r += pc.rp, sx += step, sg += step, to += step)
+                store_pack<T, VEC>(to, bw.dx(load_pack<T, VEC>(sx), load_pack<T, VEC>(sg), a.act));
+        }
     });
     pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
     share_param_grads(pl);
