@@ -19,7 +19,7 @@
 //
 // Measured (device time, 6.55 TB/s copy rate): 8 x 4800 x 256 bfloat16 with silu
 // 16.7 us forward; 16 x 76800 x 64 with relu 81.7 us; 2 x 76800 x 256 with silu
-// 46.9 us forward and 71.9 backward; 16 x 1024 x 256 padded sets 7.7 and 13.3.
+// 45.5 us forward and 72.1 backward; 16 x 1024 x 256 padded sets 7.8 and 13.3.
 //
 // Moments are kept as (mean, sum M of squared deviations) of x - pivot, the
 // pivot one of the group's values: a mean far from zero then costs its own
@@ -850,8 +850,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
 // cooperative launch, one block per SM), so the second one finds the last 160 KB
 // of every block's rows on chip and no launch lies between them.  Against two
 // launches with plain loads: 8 x 4800 x 256 18.9 -> 16.7 us, clip backward 90 ->
-// 72.  HBM bounds the way forwards, the SFU (two operations per element of
-// silu) or HBM the way back.
+// 72.  HBM bounds the way forwards (6.3 TB/s with the write-backs of earlier
+// results).  The way back of 79 MB takes 20 us: 16 without silu, 16 without the
+// stores, 16 us of HBM and L2 traffic in either case; where x exceeds L2 HBM
+// bounds it too (157 MB read and written: 6.2 TB/s).
 
 template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) {
