@@ -124,7 +124,8 @@ struct GroupOf {
 };
 
 __device__ __forceinline__ float2 mean_rstd(float pivot, float2 mean_m, int len, int Cg, float eps) {
-    const float var = len > 0 ? mean_m.y / (float(len) * float(Cg)) : 0.0f;
+    float var = len > 0 ? mean_m.y / (float(len) * float(Cg)) : 0.0f;
+    if (var < 0.0f) var = 0.0f;   // the merges' rounding of a variance next to nothing; a NaN stays one
     return make_float2(pivot + mean_m.x, 1.0f / sqrtf(var + eps));
 }
 
@@ -305,9 +306,10 @@ __global__ void __launch_bounds__(kGnThreads) gn_params_kernel(GnPlan pl) {
 //
 // For strided rows, vectors under 16 bytes and what the other forms do not
 // take.  A block reads whole rows of one chunk (a range of one sample's
-// positions).  The first sweep leaves the chunk's partial sums in the workspace, the second
-// merges its sample's partials at its start and writes the result, walking its
-// rows backwards: it begins with those that the first sweep read last.
+// positions).  The first sweep leaves the chunk's partial sums in the
+// workspace, the second merges its sample's partials at its start and writes
+// the result, walking its rows backwards: it begins with those that the first
+// sweep read last.
 
 // Valid positions of chunk k of `rows`.
 __device__ __forceinline__ int rows_of(int len, int k, int rows) { return min(max(len - k * rows, 0), rows); }

@@ -280,11 +280,28 @@ def _norm_scratch(N: int, S: int, C: int, G: int, backward: bool):
     return nbytes, (at + nbytes) // 4, at
 
 
+def _check_norm_raw(x: torch.Tensor, num_groups: int, weight, bias, lengths) -> None:
+    _need_cuda(x, "x")
+    if x.dim() < 2 or x.dtype not in _FEATURE_DTYPES:
+        raise ValueError("x must be [N, ..., C] of float32, bfloat16 or float16")
+    if num_groups < 1 or x.size(-1) % num_groups != 0:
+        raise ValueError("num_groups must be >= 1 and divide the channels")
+    both = [p for p in (weight, bias) if p is not None]
+    for p in both:
+        if p.shape != (x.size(-1),) or not p.is_contiguous() or p.dtype != both[0].dtype or \
+                p.dtype not in _FEATURE_DTYPES or p.device != x.device:
+            raise ValueError("weight and bias must be contiguous [C] of one dtype on x's device")
+    if lengths is not None and (lengths.shape != (x.size(0),) or lengths.dtype != torch.int32 or
+                                not lengths.is_contiguous() or lengths.device != x.device):
+        raise ValueError("lengths must be contiguous int32 [N] on x's device")
+
+
 def group_norm_forward_raw(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor],
                            bias: Optional[torch.Tensor], eps: float, activation: int,
                            lengths: Optional[torch.Tensor] = None):
     """One call of ``dot_group_norm_fwd`` on x [N, *S, C]; returns ``(y, stats)``: stats is a flat float32
     buffer that begins with the [N,G,2] statistics (scratch space follows)."""
+    _check_norm_raw(x, num_groups, weight, bias, lengths)
     x, N, S, C, xb, xp = _rows(x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     nbytes, nfloats, at = _norm_scratch(N, S, C, num_groups, False)
@@ -309,6 +326,11 @@ def group_norm_backward_raw(x: torch.Tensor, dy: torch.Tensor, num_groups: int, 
                             want_dweight: bool = True, want_dbias: bool = True):
     """One call of ``dot_group_norm_bwd``; returns ``(dx, dweight, dbias)``, None where not wanted (or
     where there is no such parameter)."""
+    _check_norm_raw(x, num_groups, weight, bias, lengths)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("dy must have x's shape, dtype and device")
+    if stats.dtype != torch.float32 or stats.numel() < 2 * x.size(0) * num_groups or not stats.is_contiguous():
+        raise ValueError("stats must be what group_norm_forward_raw returned")
     x, N, S, C, xb, xp = _rows(x)
     dy, _, _, _, gb, gp = _rows(dy)
     p = weight if weight is not None else bias
@@ -339,7 +361,22 @@ def rotary_raw(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: 
     """One call of ``dot_rotary`` on q [B,L,Hq,D] and/or k [B,L,Hk,D] with positions [B or 1, L, A] and
     freqs [P,A]; returns ``(q', k')``, None where the input is None."""
     ref = q if q is not None else k
+    if ref is None:
+        raise ValueError("q or k is needed")
+    for t in (q, k):
+        if t is None:
+            continue
+        _need_cuda(t, "q and k")
+        if t.dim() != 4 or t.dtype not in _FEATURE_DTYPES or t.dtype != ref.dtype or t.device != ref.device or \
+                t.shape[:2] != ref.shape[:2] or t.size(3) != ref.size(3):
+            raise ValueError("q and k must be [B, L, heads, D] of one dtype, alike but for the heads")
     B, L, _, D = ref.shape
+    if freqs.dim() != 2 or freqs.dtype != torch.float32 or not freqs.is_contiguous() or freqs.device != ref.device:
+        raise ValueError("freqs must be contiguous float32 [P, A]")
+    if positions.dim() != 3 or positions.size(0) not in (1, B) or positions.size(1) != L or \
+            positions.size(2) != freqs.size(1) or positions.dtype not in _POSITION_DTYPES or \
+            positions.device != ref.device:
+        raise ValueError("positions must be int32, int64 or float32 [B or 1, L, A]")
     qs = ks = qp = kp = qop = kop = qo = ko = None
     hq = hk = 0
     if q is not None:

@@ -520,3 +520,31 @@ def test_large_calls_on_two_streams():
                 o.append(dot.group_norm_act(x, 8, w, b))
     torch.cuda.synchronize()
     assert all(torch.equal(t, want) for o in outs for t in o)
+
+
+def test_nearly_constant_groups_without_eps():
+    """Variances down to a few roundings of the values, eps 0: finite, and within the values' own rounding."""
+    for spread in (1e-3, 1e-5, 1e-6):
+        x = (3.0 + spread * torch.randn(2, 5000, 32, generator=U.gen(7))).to(DEV)
+        y = dot.group_norm_act(x, 4, eps=0.0, activation="none")
+        want = norm64(x.double(), 4, None, None, 0.0, "none")
+        assert torch.isfinite(y).all()
+        # the stored mean is off by up to 3 * 2^-23 of the smallest standard deviation
+        std = float(x.double().reshape(2, 5000, 4, 8).std(dim=(1, 3)).min())
+        assert float((y.double() - want).abs().max()) <= 2.0 ** -22 / std + 1e-4 * float(want.abs().max())
+
+
+def test_raw_refusals():
+    from dot_b200 import ops
+
+    x, w = torch.randn(2, 10, 32, device=DEV), torch.ones(32, device=DEV)
+    y, stats = ops.group_norm_forward_raw(x, 4, w, None, 1e-5, 1)
+    for bad in (lambda: ops.group_norm_forward_raw(x, 5, w, None, 1e-5, 1),
+                lambda: ops.group_norm_forward_raw(x, 4, w[:16], None, 1e-5, 1),
+                lambda: ops.group_norm_forward_raw(x, 4, w, w.half(), 1e-5, 1),
+                lambda: ops.group_norm_forward_raw(x, 4, w, None, 1e-5, 1, torch.ones(2, device=DEV)),
+                lambda: ops.group_norm_backward_raw(x, y.half(), 4, w, None, 1, stats),
+                lambda: ops.group_norm_backward_raw(x, y[:1], 4, w, None, 1, stats),
+                lambda: ops.group_norm_backward_raw(x, y, 4, w, None, 1, stats[:4])):
+        with pytest.raises(ValueError):
+            bad()

@@ -306,3 +306,19 @@ def test_single_calls_of_the_c_abi():
     got = ops.rotary_raw(q, k, pos.unsqueeze(0), freqs, False)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(ops.rotary_raw(None, k, pos.unsqueeze(0), freqs, False)[1], want[1])
+
+
+def test_raw_refusals():
+    from dot_b200 import ops
+
+    q, pos, freqs = rand(2, 10, 4, 32), torch.zeros(2, 10, 2, device=DEV), table(16, 2)
+    for bad in (lambda: ops.rotary_raw(None, None, pos, freqs, False),
+                lambda: ops.rotary_raw(q[0], None, pos, freqs, False),
+                lambda: ops.rotary_raw(q, q[:, :5], pos, freqs, False),
+                lambda: ops.rotary_raw(q, q.half(), pos, freqs, False),
+                lambda: ops.rotary_raw(q, None, pos[:, :9], freqs, False),
+                lambda: ops.rotary_raw(q, None, pos.double(), freqs, False),
+                lambda: ops.rotary_raw(q, None, pos, freqs[:, :1], False),
+                lambda: ops.rotary_raw(q, None, pos, table(17, 2), False)):
+        with pytest.raises(ValueError):
+            bad()
