@@ -19,7 +19,7 @@
 //
 // Measured (device time, 6.55 TB/s copy rate): 8 x 4800 x 256 bfloat16 with silu
 // 16.7 us forward; 16 x 76800 x 64 with relu 81.7 us; 2 x 76800 x 256 with silu
-// 45.5 us forward and 72.1 backward; 16 x 1024 x 256 padded sets 7.8 and 13.3.
+// 45.5 us forward and 72.1 backward; 16 x 1024 x 256 padded sets 7.8 and 14.1.
 //
 // Moments are kept as (mean, sum M of squared deviations) of x - pivot, the
 // pivot one of the group's values: a mean far from zero then costs its own
@@ -29,6 +29,7 @@
 // (Chan, Golub and LeVeque, 1979); threads' and blocks' pairs are joined by Merge.
 #pragma once
 
+#include <atomic>
 #include <cooperative_groups.h>
 
 #include "cluster.cuh"
@@ -61,6 +62,7 @@ struct GnPlan {
     int rows;            // positions per chunk
     int slab_groups;     // resident: groups of a block's channel slab
     int slabs;           // resident: slabs per sample
+    int share;           // resident, bwd: the blocks meet at the end and sum the parameters' gradients
     float2* moments;     // sweeps, fwd: [N][chunks][G] (mean, M) of a chunk
     float2* gsums;       // sweeps, bwd: [N][chunks][G] (sum w dz, sum w dz xh)
     float2* csums;       // bwd: [N][chunks][C] (sum dz, sum dz xh)
@@ -268,13 +270,13 @@ struct BackwardDx : Backward<T, VEC, ACT, ONEG> {
 
 // ---- backward: the parameters' gradients from the blocks' channel sums ---------
 
-// Channels c = first + warp, + kGnWarps, ... < end: a warp sums a channel's
+// Channels c = first + warp, + the block's warps, ... < end: a warp sums a channel's
 // pairs over all samples' chunks, in an order that depends on nothing else.
 __device__ __forceinline__ void param_grads(const GnPlan& pl, int first, int end) {
     const GroupNormArgs& a = pl.a;
     const int C = int(a.C), lane = threadIdx.x & 31;
     const int64_t rows = a.N * pl.chunks;
-    for (int c = first + int(threadIdx.x >> 5); c < end; c += kGnWarps) {
+    for (int c = first + int(threadIdx.x >> 5); c < end; c += int(blockDim.x) / 32) {
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 4
         for (int64_t r = lane; r < rows; r += 32) {
@@ -1036,9 +1038,12 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
 // A cluster of `chunks` blocks holds one sample's positions of one channel slab
 // (whole groups) in registers: x (and dy) are read once, the blocks exchange
 // their groups' partial sums through distributed shared memory, and the result
-// is written from the registers.  One launch per direction (and a small one for
-// the parameters' gradients, which cross clusters).  Bound by latency: 3.4 us
-// for one 64 x 64 sample, 7.7 us forward and 13.3 us backward for 8.4 MB.
+// is written from the registers.  One launch per direction: the parameters'
+// gradients, which cross clusters, follow a grid barrier at the end where all
+// clusters run at once (a launch of their own costs a training call 7 us of 73
+// on the host and saves 1 us of 14 on the device), else they are a second
+// launch.  Bound by latency: 3.4 us for one 64 x 64 sample, 7.8 us forward and
+// 14.1 us backward for 8.4 MB.
 
 // Where a block stands: chunk (its rank in the cluster), slab, sample.
 struct ResPlace {
@@ -1248,6 +1253,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_resident_bwd_kernel(GnPlan p
         }
     }
     if (pl.chunks > 1) cl_wait();     // no block leaves while a peer may read its sums
+    if (pl.share) {
+        cooperative_groups::this_grid().sync();
+        share_param_grads(pl);
+    }
 }
 
 // ---- host ---------------------------------------------------------------------
@@ -1302,6 +1311,34 @@ bool cooperative_device() {
         known[dev] = sms >= kSMs && coop ? 1 : -1;
     }
     return known[dev] > 0;
+}
+
+// Whether a launch's clusters can all run at the same time, so that its blocks
+// may wait for one another (asked once for each kernel and cluster size).
+template <void (*kernel)(GnPlan)>
+bool all_at_once(int64_t blocks, int threads, size_t smem, int cluster) {
+    if (!cooperative_device()) return false;
+    if (cluster == 1) return blocks <= kSMs;
+    static std::atomic<int> known[kMaxCluster + 1];   // this kernel's clusters of each size; 0: not asked yet
+    int most = known[cluster].load(std::memory_order_relaxed);
+    if (most == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(cluster * kSMs));
+        cfg.blockDim = dim3(unsigned(kGnThreads));
+        cfg.dynamicSmemBytes = 48 * 1024;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(cluster);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most <= 0) {
+            cudaGetLastError();
+            most = -1;
+        }
+        known[cluster].store(most, std::memory_order_relaxed);
+    }
+    return threads <= kGnThreads && smem <= 48 * 1024 && blocks / cluster <= most;
 }
 
 template <typename K>
@@ -1391,10 +1428,13 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
     int rc = DOT_OK;
     if constexpr (KV <= res_vecs(VEC * sizeof(T), true)) {
         carve(ws, pl, true);
+        constexpr auto kernel = gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>;
+        pl.share = (pl.a.dweight || pl.a.dbias) && all_at_once<kernel>(blocks, threads, smem, pl.chunks);
         ProfScope ps(DOT_K_NORM_BWD, st);
-        rc = launch(gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, kPlain, st);
+        rc = launch(kernel, pl, blocks, threads, smem, pl.chunks, pl.share ? kCooperative : kPlain, st);
     }
-    return rc ? rc : launch_params(pl, st);
+    if (rc || pl.share) return rc;
+    return launch_params(pl, st);
 }
 
 template <typename T, int VEC, int ACT, bool ONEG>
