@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/dot_b200.h"
@@ -35,6 +36,17 @@ void check(int rc, const char* what) {
     TORCH_CHECK_NOT_IMPLEMENTED(rc != DOT_ERR_UNSUPPORTED, what, ": ", msg);
     TORCH_CHECK_VALUE(rc != DOT_ERR_INVALID, what, ": ", msg);
     TORCH_CHECK(false, what, " failed (", rc, "): ", msg);
+}
+
+// What would pass these operators by without a word is refused: a tangent of forward-mode
+// differentiation would be dropped, and a trace would keep the allocation of the outputs
+// but not the launch that fills them.
+template <typename... Ts>
+void refuse_modes(const char* what, const Ts&... inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "dot_b200: ", what,
+                                " cannot be recorded by torch.jit.trace");
+    const bool tangent = ((inputs.defined() && inputs._fw_grad(/*level=*/0).defined()) || ...);
+    TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "dot_b200: ", what, " has no forward-mode derivative");
 }
 
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -119,6 +131,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &lengths = saved[3], &stats = saved[4];
+        refuse_modes("the backward of group_norm_act", grads[0]);
         const int64_t groups = ctx->saved_data["groups"].toInt(), act = ctx->saved_data["activation"].toInt();
         const Rows r(x), g(grads[0]);
         const c10::cuda::CUDAGuard guard(x.device());
@@ -162,6 +175,7 @@ Tensor norm_param(const optional<Tensor>& p, const Tensor& x, const char* name) 
 
 Tensor group_norm_act(const Tensor& x, int64_t groups, const optional<Tensor>& weight, const optional<Tensor>& bias,
                       double eps, int64_t activation, const optional<Tensor>& lengths_in) {
+    refuse_modes("group_norm_act", x, weight.value_or(Tensor()), bias.value_or(Tensor()));
     TORCH_CHECK(x.is_cuda(), "dot_b200: x must be a CUDA tensor (dot_b200 runs on NVIDIA GPUs only)");
     TORCH_CHECK_VALUE(x.dim() >= 2, "x must be [N, ..., C]");
     TORCH_CHECK_NOT_IMPLEMENTED(feature_dtype(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ",
@@ -256,6 +270,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
         if (ctx->saved_data["has_k"].toBool() && ctx->needs_input_grad(input)) dk = grads[input];
         variable_list all(6);
         if (!dq.defined() && !dk.defined()) return all;
+        refuse_modes("the backward of rotary", dq, dk);
         // the turn is orthogonal: its backward is the turn by -angle
         if (at::GradMode::is_enabled()) {
             variable_list outs = RotaryFn::apply(present(dq), present(dk), saved[0], saved[1], interleaved, !inverse);
@@ -286,6 +301,7 @@ Tensor as_4d(const Tensor& x) {
 
 std::pair<Tensor, optional<Tensor>> rotary(const Tensor& q, const Tensor& positions_in, const Tensor& freqs_in,
                                            const optional<Tensor>& k_in, bool interleaved) {
+    refuse_modes("rotary", q, k_in.value_or(Tensor()), positions_in, freqs_in);
     check_heads(q, "q");
     const int64_t dims = q.dim(), lead = dims - 2, L = q.size(-3), D = q.size(-1);
     Tensor k;

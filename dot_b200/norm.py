@@ -50,7 +50,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     ``activation``: "silu", "gelu" (the erf form), "relu" or "none".
     ``weight``, ``bias``: [C], float32 or a 16-bit type.  ``lengths``: int32
     [N], valid positions of each sample in the flattened position axes.
-    Gradients for x, weight and bias (once differentiable).
+    Gradients for x, weight and bias (once differentiable, in reverse mode);
+    forward-mode tangents and ``torch.jit.trace`` raise NotImplementedError.
     """
     return _binding.group_norm_act(x, num_groups, weight, bias, eps, _activation_code(activation), lengths)
 

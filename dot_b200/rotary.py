@@ -36,7 +36,8 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Opt
     2 P <= D; elements from 2 P on pass through.  Pair p is (x_p, x_{P+p}), or
     (x_2p, x_2p+1) with ``interleaved``.  q and k may be slices of wider rows
     (a fused projection); the results are dense.  Returns q', or (q', k') when
-    k is given.  Differentiable in q and k, not in positions or freqs.
+    k is given.  Differentiable in q and k, not in positions or freqs;
+    forward-mode tangents and ``torch.jit.trace`` raise NotImplementedError.
     """
     q, turned_k = _binding.rotary(q, positions, freqs, k, interleaved)
     return q if k is None else (q, turned_k)
