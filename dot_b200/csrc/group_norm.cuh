@@ -334,11 +334,19 @@ struct Place {
 // forwards and then backwards: up to 160 KB in flight per SM without a
 // register, and the way back begins with the stages that are still there.  A
 // stage holds U rows for each row position of the block, of x and for NT = 2 of
-// dy; the last of the 16 warps to leave a stage refills it.  Waits are bounded:
-// one that expires makes the block go on without waiting, and its results are
-// written as NaN.
+// dy; the last of the 16 warps to leave a stage refills it.  Waits are bounded.
+// A thread whose wait expired goes on without waiting and writes NaN, into every
+// channel of its partial sums on the way in and of its rows on the way out; the
+// block starts no further copy, since the barrier of the lost one is still in its
+// phase, and before it ends waits (again with a limit) for those in flight.
 constexpr int kRingStages = 5;
 constexpr int kRingStageBytes = 32 * 1024;
+
+// Whether the c-th copy into stage i's slot is left out: never, but for the test of
+// the expired wait, which defines it before including this file.
+#ifndef DOTB_RING_LOSES
+#define DOTB_RING_LOSES(i, c) false
+#endif
 
 template <int NT>
 struct Ring {
@@ -346,18 +354,23 @@ struct Ring {
     unsigned char* buf;
     uint64_t* full;                     // [kRingStages]
     int* left;                          // [kRingStages] warps that have left the stage
+    int* copies;                        // [kRingStages] copies started into the slot
+    volatile int* lost;                 // a wait expired: no copy is started any more
     const unsigned char* src[NT];       // row 0 of the block's range
     int row_bytes, rows, stage_rows, n; // rows in all, per stage; stages
     bool dead = false;
 
     static constexpr size_t bytes() {   // what follows is 16-byte aligned
-        return (size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + sizeof(int)) + 15) / 16 * 16;
+        const size_t stage = kRingStageBytes + sizeof(uint64_t) + 2 * sizeof(int);
+        return (size_t(kRingStages) * stage + sizeof(int) + 15) / 16 * 16;
     }
     // By all threads, before a block barrier.
     __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_) {
         buf = smem;
         full = reinterpret_cast<uint64_t*>(smem + kRingStages * kRingStageBytes);
         left = reinterpret_cast<int*>(full + kRingStages);
+        copies = left + kRingStages;
+        lost = copies + kRingStages;
         rows = rows_;
         stage_rows = stage_rows_;
         row_bytes = row_bytes_;
@@ -366,16 +379,20 @@ struct Ring {
 #pragma unroll
             for (int k = 0; k < kRingStages; ++k) {
                 mbar_init(full + k, 1);
-                left[k] = 0;
+                left[k] = copies[k] = 0;
             }
+            *lost = 0;
             mbar_fence_init();
         }
     }
     // Stage i holds rows [i stage_rows, + count(i)).
     __device__ __forceinline__ int count(int i) const { return min(stage_rows, rows - i * stage_rows); }
-    __device__ __forceinline__ void issue(int i) {
+    // Stage i as the c-th copy into its slot.
+    __device__ __forceinline__ void issue(int i, int c) {
         const int slot = i % kRingStages;
         const uint32_t bytes = uint32_t(count(i)) * uint32_t(row_bytes);
+        if (DOTB_RING_LOSES(i, c)) return;
+        copies[slot] = c + 1;
         mbar_arrive_expect_tx(full + slot, NT * bytes);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -385,10 +402,10 @@ struct Ring {
     // After that barrier.
     __device__ __forceinline__ void fill() {
         if (threadIdx.x == 0)
-            for (int i = 0; i < min(n, kRingStages); ++i) issue(i);
+            for (int i = 0; i < min(n, kRingStages); ++i) issue(i, 0);
     }
-    // A warp leaves stage i; the last one brings stage `next` into its place.
-    __device__ __forceinline__ void leave(int i, int next) {
+    // A warp leaves stage i; the last one brings stage `next` into its place, its c-th copy.
+    __device__ __forceinline__ void leave(int i, int next, int c) {
         const int slot = i % kRingStages;
         __syncwarp();
         if ((threadIdx.x & 31) == 0) {
@@ -397,9 +414,14 @@ struct Ring {
                 left[slot] = 0;
                 __threadfence_block();
                 fence_proxy_async_smem();
-                issue(next);
+                if (!*lost) issue(next, c);   // set before the warp that set it left
             }
         }
+    }
+    __device__ __forceinline__ void wait(int i) {
+        if (dead || mbar_wait_sleep(full + i % kRingStages, uint32_t(i / kRingStages) & 1u, nullptr)) return;
+        dead = true;
+        *lost = 1;
     }
     // use(stage's bytes, its first row, its rows), first stage to last.  The
     // c-th copy into a slot completes its barrier's phase c: stage i is copy
@@ -407,26 +429,41 @@ struct Ring {
     template <typename F>
     __device__ __forceinline__ void forwards(F use) {
         for (int i = 0; i < n; ++i) {
-            const int slot = i % kRingStages;
-            if (!dead) dead = !mbar_wait_sleep(full + slot, uint32_t(i / kRingStages) & 1u, nullptr);
-            use(buf + slot * kRingStageBytes, i * stage_rows, count(i));
-            if (i + kRingStages < n) leave(i, i + kRingStages);
+            wait(i);
+            use(buf + (i % kRingStages) * kRingStageBytes, i * stage_rows, count(i));
+            if (i + kRingStages < n) leave(i, i + kRingStages, i / kRingStages + 1);
         }
     }
     // ... and, m = (slot's last stage) / kRingStages, copy 2 m - i / kRingStages
-    // on the way back, which has the same parity.  The last stages are still there.
+    // on the way back, which has the same parity (the stage below it in the slot is
+    // one copy more).  The last stages are still there.
     template <typename F>
     __device__ __forceinline__ void backwards(F use) {
         for (int i = n - 1; i >= 0; --i) {
-            const int slot = i % kRingStages;
-            if (!dead && i < n - kRingStages) dead = !mbar_wait_sleep(full + slot, uint32_t(i / kRingStages) & 1u, nullptr);
-            use(buf + slot * kRingStageBytes, i * stage_rows, count(i));
-            if (i >= kRingStages) leave(i, i - kRingStages);
+            if (i < n - kRingStages) wait(i);
+            use(buf + (i % kRingStages) * kRingStageBytes, i * stage_rows, count(i));
+            if (i >= kRingStages)
+                leave(i, i - kRingStages, (n - 1 - i % kRingStages) / kRingStages * 2 - i / kRingStages + 1);
         }
-        if (dead)   // copies still in flight must not outlive the block; the last into a slot is an even one
-            for (int k = 0; k < min(n, kRingStages); ++k) mbar_wait_sleep(full + k, 0u, nullptr);
+    }
+    // At the end, by all threads: copies still in flight must not outlive the block.
+    __device__ __forceinline__ void drain() {
+        if (__syncthreads_or(dead) && threadIdx.x < kRingStages && copies[threadIdx.x] > 0)
+            mbar_wait_sleep(full + threadIdx.x, uint32_t(copies[threadIdx.x] - 1) & 1u, nullptr);
     }
 };
+
+// NaN for what an expired wait left without its data.
+template <int N>
+__device__ __forceinline__ void poison(float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __int_as_float(0x7fffffff);
+}
+template <int N>
+__device__ __forceinline__ void poison(float2 (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = splat2(__int_as_float(0x7fffffff));
+}
 
 // Mean (about the pivot) and M of the first `k` of U vectors of a thread, per
 // channel, or one for all channels of a vector that lies in one group: two
@@ -903,7 +940,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
                 run.join(bt, float(k));
             }
         });
-        if (ring.dead) run.mean[0] = __int_as_float(0x7fffffff);
+        if (ring.dead) poison(run.mean);
         if (pc.on)
 #pragma unroll
             for (int j = 0; j < W; ++j) part[(pc.r * pc.nv + pc.v) * W + j] = make_float2(run.mean[j], run.m2[j]);
@@ -923,7 +960,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
     T* y = static_cast<T*>(a.y) + int64_t(n) * a.S * C;
     if (pc.on) fw.stats(c, Cg, acc);
     ring.backwards([&](const unsigned char* sx, int first, int rows) {
-        if (ring.dead) fw.scale[0] = splat2(__int_as_float(0x7fffffff));
+        if (ring.dead) poison(fw.scale);
         const T* at = reinterpret_cast<const T*>(sx) + pc.r * C + c;
         T* to = y + int64_t(p0 + first + pc.r) * C + c;
         if (!pc.on) return;
@@ -941,6 +978,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_fwd_kernel(GnPlan pl) 
         }
     });
     pad_rows<T, VEC>(pc, y, C, c, pv, pe);
+    ring.drain();
 }
 
 template <typename T, int VEC, int ACT, bool ONEG>
@@ -996,7 +1034,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
                     bw.sums(load_pack<T, VEC>(sx), load_pack<T, VEC>(sg), a.act, sa, sb);
             }
         });
-        if (ring.dead) sa[0] = splat2(__int_as_float(0x7fffffff));
+        if (ring.dead) {
+            poison(sa);
+            poison(sb);
+        }
         if (pc.on) put_pairs<VEC>(part + (pc.r * pc.nv + pc.v) * VEC, sa, sb);
     }
     __syncthreads();
@@ -1008,7 +1049,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
     if (pc.on) bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
     ring.backwards([&](const unsigned char* s0, int first, int rows) {
-        if (ring.dead) bw.rw[0] = splat2(__int_as_float(0x7fffffff));
+        if (ring.dead) poison(bw.rw);
         const T* sx = reinterpret_cast<const T*>(s0) + pc.r * C + c;
         const T* sg = reinterpret_cast<const T*>(s0 + Ring<2>::kPart) + pc.r * C + c;
         T* to = dx + int64_t(p0 + first + pc.r) * C + c;
@@ -1031,6 +1072,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     });
     pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
     share_param_grads(pl);
+    ring.drain();
 }
 
 // ---- resident path ------------------------------------------------------------

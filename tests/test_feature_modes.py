@@ -50,7 +50,8 @@ def test_traces_are_refused(device, i):
 
 @pytest.mark.gpu
 def test_tangents_of_upstream_gradients_are_refused():
-    x, q = torch.rand(2, 3, 8, device="cuda", requires_grad=True), torch.rand(1, 3, 2, 8, device="cuda", requires_grad=True)
+    x = torch.rand(2, 3, 8, device="cuda", requires_grad=True)
+    q = torch.rand(1, 3, 2, 8, device="cuda", requires_grad=True)
     for leaf, y in ((x, dot.group_norm_act(x, 2)), (q, dot.rotary(q, POS.cuda(), FREQS.cuda()))):
         with fw.dual_level():
             up = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
