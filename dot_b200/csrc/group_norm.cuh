@@ -50,6 +50,15 @@ constexpr int kGnThreads = 512;
 constexpr int kGnWarps = kGnThreads / 32;
 constexpr int kMaxCluster = 8;
 
+// Shared memory: what a block may have, what it has without asking, and what the
+// merges over a sample's chunks (sample_stats, sample_sums) hold beside the
+// dynamic part.  The sweeps' groups are bounded by it: 8 bytes each next to those
+// merges in the second sweep, next to the threads' pairs in the first (fits()).
+constexpr size_t kSmemMost = 227 * 1024, kSmemDefault = 48 * 1024;
+constexpr size_t kSmemMerges = size_t(kGnWarps) * 32 * sizeof(float2);
+constexpr int64_t kMaxGroups = int64_t((kSmemMost - kSmemMerges) / sizeof(float2));
+static_assert((size_t(kMaxGroups) + kGnThreads) * sizeof(float2) <= kSmemMost, "vectors of one element take any G");
+
 // Resident path: vectors that a thread keeps of x (forward), or of x and of dy.
 constexpr int res_vecs(int bytes, bool backward) {
     const int n = bytes >= 16 ? 8 : bytes >= 8 ? 16 : 32;
@@ -589,6 +598,7 @@ __device__ __forceinline__ void tile_moments(const Place& pc, int tile, int Cg, 
 template <typename F>
 __device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write, int len, F pivot, float2* st) {
     __shared__ Merge merged[kGnWarps][32];
+    static_assert(sizeof(merged) == kSmemMerges, "counted by launch()");
     const GroupNormArgs& a = pl.a;
     const int G = int(a.G), Cg = int(a.C) / G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the chunks
@@ -652,11 +662,12 @@ __device__ __forceinline__ void tile_sums(const GnPlan& pl, const Place& pc, int
     }
 }
 
-// Mean, rstd, S1/m and S2/m [G] of sample n from its chunks' sums, by the whole
-// block; stats(g): mean and rstd of group g.
+// S1/m and S2/m of sample n's groups from its chunks' sums, by the whole block;
+// put(g, pair) takes group g's.
 template <typename F>
-__device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, F stats, float4* gv) {
+__device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, F put) {
     __shared__ float2 merged[kGnWarps][32];
+    static_assert(sizeof(merged) == kSmemMerges, "counted by launch()");
     const GroupNormArgs& a = pl.a;
     const int C = int(a.C), G = int(a.G), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv = len > 0 ? 1.0f / (float(len) * float(C / G)) : 0.0f;
@@ -677,8 +688,7 @@ __device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, F 
                 s.x += merged[k][lane].x;
                 s.y += merged[k][lane].y;
             }
-            const float2 v = stats(g);
-            gv[g] = make_float4(v.x, v.y, s.x * inv, s.y * inv);
+            put(g, make_float2(s.x * inv, s.y * inv));
         }
         __syncthreads();
     }
@@ -843,14 +853,14 @@ template <typename T, int VEC, int ACT, bool ONEG>
 __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
     const GroupNormArgs& a = pl.a;
     extern __shared__ float gn_smem[];
-    float4* gv = reinterpret_cast<float4*>(gn_smem);   // [G] mean, rstd, S1/m, S2/m
+    float2* sums = reinterpret_cast<float2*>(gn_smem);   // [G] S1/m, S2/m
     constexpr int U = 4;
     const int C = int(a.C), Cg = C / int(a.G), cv = C / VEC;
     const int n = int(blockIdx.x) / pl.chunks, chunk = int(blockIdx.x) % pl.chunks;
     const int len = valid_len(a, n);
     pdl_launch_dependents();
     pdl_wait();
-    sample_sums(pl, n, len, [&](int g) { return reinterpret_cast<const float2*>(a.stats)[int64_t(n) * a.G + g]; }, gv);
+    sample_sums(pl, n, len, [&](int g, float2 s) { sums[g] = s; });
     const int p0 = chunk * pl.rows, pe = min(int(a.S), p0 + pl.rows), pv = min(max(len, p0), pe);
     const T* x = static_cast<const T*>(a.x) + int64_t(n) * a.xb;
     const T* dy = static_cast<const T*>(a.dy) + int64_t(n) * a.gb;
@@ -860,8 +870,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
         if (!pc.on) continue;
         const int c = (tile * kGnThreads + pc.v) * VEC;
         BackwardDx<T, VEC, ACT, ONEG> bw;
-        bw.load(a, c, c, Cg, gv);
-        bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
+        bw.load(a, c, c, Cg, reinterpret_cast<const float2*>(a.stats) + int64_t(n) * a.G);
+        bw.finish(c, Cg, len, [&](int g) { return sums[g]; });
         pad_rows<T, VEC>(pc, dx, C, c, pv, pe);
         int left = max(0, pv - p0 - pc.r + pc.rp - 1) / pc.rp;
         const T* xc = x + int64_t(pv - 1 - pc.r) * a.xp + c;
@@ -1045,7 +1055,7 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
     __syncthreads();
     for (int g = threadIdx.x; g < G; g += kGnThreads) pl.gsums[slot * G + g] = acc[g];
     cooperative_groups::this_grid().sync();   // the parameters' gradients need every block's sums
-    sample_sums(pl, n, len, [&](int g) { return make_float2(gv[g].x, gv[g].y); }, gv);
+    sample_sums(pl, n, len, [&](int g, float2 s) { gv[g] = make_float4(gv[g].x, gv[g].y, s.x, s.y); });
     T* dx = static_cast<T*>(a.dx) + int64_t(n) * a.S * C;
     if (pc.on) bw.finish(c, Cg, len, [&](int g) { return make_float2(gv[g].z, gv[g].w); });
     ring.backwards([&](const unsigned char* s0, int first, int rows) {
@@ -1387,11 +1397,9 @@ template <typename K>
 int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem, int cluster, LaunchKind kind,
            cudaStream_t st) {
     if (blocks > 0x7fffffff) return fail(DOT_ERR_UNSUPPORTED, "group norm: too many blocks");
-    if (smem > 48 * 1024) {
-        if (smem > 227 * 1024) return fail(DOT_ERR_UNSUPPORTED, "group norm: too many groups");
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-            return check_launch("group norm");
-    }
+    if (smem + kSmemMerges > kSmemDefault &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+        return check_launch("group norm");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(blocks));
     cfg.blockDim = dim3(unsigned(threads));
@@ -1486,7 +1494,7 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     carve(ws, pl, backward);
     const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1);
     const size_t s1 = (size_t(a.G) + part) * sizeof(float2);
-    const size_t s2 = size_t(a.G) * (backward ? sizeof(float4) : sizeof(float2));
+    const size_t s2 = size_t(a.G) * sizeof(float2);
     const int64_t blocks = a.N * pl.chunks;
     const bool second = !backward || a.dx != nullptr;
     int rc;
@@ -1565,8 +1573,10 @@ int by_act(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st) {
     }
 }
 
-// Whether vectors of `vec` elements of `esz` bytes are aligned in every tensor.
+// Whether vectors of `vec` elements of `esz` bytes are aligned in every tensor, and
+// a block's pairs of them leave the groups' their shared memory.
 bool fits(const GroupNormArgs& a, int vec, int esz) {
+    if (size_t(a.G + int64_t(kGnThreads) * vec) * sizeof(float2) > kSmemMost) return false;
     const int64_t bytes = int64_t(vec) * esz;
     auto ok = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
     if (a.C % vec || a.xb % vec || a.xp % vec || a.gb % vec || a.gp % vec) return false;
@@ -1575,6 +1585,7 @@ bool fits(const GroupNormArgs& a, int vec, int esz) {
 
 template <typename T>
 int by_width(const GroupNormArgs& a, void* ws, bool backward, cudaStream_t st) {
+    if (a.G > kMaxGroups) return fail(DOT_ERR_UNSUPPORTED, "more than " + std::to_string(kMaxGroups) + " groups");
     if constexpr (sizeof(T) == 2)
         if (fits(a, 8, 2)) return by_act<T, 8>(a, ws, backward, st);
     if (fits(a, 4, sizeof(T))) return by_act<T, 4>(a, ws, backward, st);

@@ -47,6 +47,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
                    lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Group norm and activation of ``x`` [N, *S, C]; returns a dense tensor of x's shape and dtype.
 
+    ``num_groups``: divides C, at most 28544.
     ``activation``: "silu", "gelu" (the erf form), "relu" or "none".
     ``weight``, ``bias``: [C], float32 or a 16-bit type.  ``lengths``: int32
     [N], valid positions of each sample in the flattened position axes.

@@ -380,7 +380,8 @@ DOT_API size_t dot_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t 
  * x: S positions of C consecutive elements per sample, x_batch_stride and
  * x_pos_stride elements from one sample / position to the next (a slice of
  * wider rows is read in place); y is dense [N,S,C] of x's dtype (DOT_F32,
- * DOT_BF16 or DOT_F16; computed in fp32, rounded once).  weight, bias [C] of
+ * DOT_BF16 or DOT_F16; computed in fp32, rounded once).  G is at most 28544
+ * (DOT_ERR_UNSUPPORTED beyond, forward and backward alike).  weight, bias [C] of
  * param_dtype (each may be NULL: 1 and 0).  lengths: device int32 [N], clamped
  * to [0, S] (NULL: all S).  stats [N,G,2] fp32 receives (mean,
  * 1/sqrt(var + eps)) for the backward ((0, 1/sqrt(eps)) where nothing is valid).
