@@ -598,7 +598,7 @@ __device__ __forceinline__ void tile_moments(const Place& pc, int tile, int Cg, 
 template <typename F>
 __device__ __forceinline__ void sample_stats(const GnPlan& pl, int n, bool write, int len, F pivot, float2* st) {
     __shared__ Merge merged[kGnWarps][32];
-    static_assert(sizeof(merged) == kSmemMerges, "counted by launch()");
+    static_assert(sizeof(merged) == kSmemMerges, "as launch() is told");
     const GroupNormArgs& a = pl.a;
     const int G = int(a.G), Cg = int(a.C) / G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int g = lane; g < (G + 31) / 32 * 32; g += 32) {   // a lane a group, the warps share the chunks
@@ -667,7 +667,7 @@ __device__ __forceinline__ void tile_sums(const GnPlan& pl, const Place& pc, int
 template <typename F>
 __device__ __forceinline__ void sample_sums(const GnPlan& pl, int n, int len, F put) {
     __shared__ float2 merged[kGnWarps][32];
-    static_assert(sizeof(merged) == kSmemMerges, "counted by launch()");
+    static_assert(sizeof(merged) == kSmemMerges, "as launch() is told");
     const GroupNormArgs& a = pl.a;
     const int C = int(a.C), G = int(a.G), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv = len > 0 ? 1.0f / (float(len) * float(C / G)) : 0.0f;
@@ -1393,12 +1393,15 @@ bool all_at_once(int64_t blocks, int threads, size_t smem, int cluster) {
     return threads <= kGnThreads && smem <= 48 * 1024 && blocks / cluster <= most;
 }
 
+// smem: dynamic, beside `merges` static bytes.  The opt-in is the kernel's and not the
+// launch's: all calls, from any thread, set it to the same most.
 template <typename K>
-int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem, int cluster, LaunchKind kind,
-           cudaStream_t st) {
+int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem, size_t merges, int cluster,
+           LaunchKind kind, cudaStream_t st) {
     if (blocks > 0x7fffffff) return fail(DOT_ERR_UNSUPPORTED, "group norm: too many blocks");
-    if (smem + kSmemMerges > kSmemDefault &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    if (smem + merges > kSmemDefault &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemMost - merges)) !=
+            cudaSuccess)
         return check_launch("group norm");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(blocks));
@@ -1432,7 +1435,7 @@ int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem,
 int launch_params(const GnPlan& pl, cudaStream_t st) {
     if (!pl.a.dweight && !pl.a.dbias) return DOT_OK;
     ProfScope ps(DOT_K_NORM_BWD, st);
-    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, kGnWarps), kGnThreads, 0, 1, kDependent, st);
+    return launch(gn_params_kernel, pl, ceil_div(pl.a.C, kGnWarps), kGnThreads, 0, 0, 1, kDependent, st);
 }
 
 // The resident plan of a problem, if its blocks hold it in registers all at
@@ -1473,7 +1476,8 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
     const int64_t blocks = pl.a.N * pl.slabs * pl.chunks;
     if (!backward) {
         ProfScope ps(DOT_K_NORM_FWD, st);
-        return launch(gn_resident_fwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, pl.chunks, kPlain, st);
+        return launch(gn_resident_fwd_kernel<T, VEC, ACT, ONEG, KV>, pl, blocks, threads, smem, 0, pl.chunks, kPlain,
+                      st);
     }
     int rc = DOT_OK;
     if constexpr (KV <= res_vecs(VEC * sizeof(T), true)) {
@@ -1481,7 +1485,7 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
         constexpr auto kernel = gn_resident_bwd_kernel<T, VEC, ACT, ONEG, KV>;
         pl.share = (pl.a.dweight || pl.a.dbias) && all_at_once<kernel>(blocks, threads, smem, pl.chunks);
         ProfScope ps(DOT_K_NORM_BWD, st);
-        rc = launch(kernel, pl, blocks, threads, smem, pl.chunks, pl.share ? kCooperative : kPlain, st);
+        rc = launch(kernel, pl, blocks, threads, smem, 0, pl.chunks, pl.share ? kCooperative : kPlain, st);
     }
     if (rc || pl.share) return rc;
     return launch_params(pl, st);
@@ -1500,11 +1504,13 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
     int rc;
     {
         ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st, second ? 2 : 1);
-        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 1, kPlain, st)
-                      : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 1, kPlain, st);
+        rc = backward ? launch(gn_sums_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s1, 0, 1, kPlain, st)
+                      : launch(gn_moments_kernel<T, VEC, ONEG>, pl, blocks, kGnThreads, s1, 0, 1, kPlain, st);
         if (!rc && second)
-            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, kDependent, st)
-                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, 1, kDependent, st);
+            rc = backward ? launch(gn_dx_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, kSmemMerges, 1,
+                                   kDependent, st)
+                          : launch(gn_apply_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads, s2, kSmemMerges, 1,
+                                   kDependent, st);
     }
     if (rc) return rc;
     return backward && !second ? launch_params(pl, st) : DOT_OK;
@@ -1527,9 +1533,9 @@ bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
     const size_t groups = size_t(a.G + 1) * (backward ? sizeof(float4) + sizeof(float2) : sizeof(float2) + sizeof(float));
     ProfScope ps(backward ? DOT_K_NORM_BWD : DOT_K_NORM_FWD, st);
     rc = backward ? launch(gn_fused_bwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
-                           Ring<2>::bytes() + groups + part, 1, kCooperative, st)
+                           Ring<2>::bytes() + groups + part, kSmemMerges, 1, kCooperative, st)
                   : launch(gn_fused_fwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
-                           Ring<1>::bytes() + groups + part, 1, waits ? kCooperative : kPlain, st);
+                           Ring<1>::bytes() + groups + part, kSmemMerges, 1, waits ? kCooperative : kPlain, st);
     return true;
 }
 
