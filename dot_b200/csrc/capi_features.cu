@@ -12,6 +12,22 @@ namespace {
 
 bool float_dtype(int d) { return d == DOT_F32 || d == DOT_BF16 || d == DOT_F16; }
 
+// Whether every address (NULL among them) is a multiple of `bytes`: the kernels read
+// pairs and single elements whatever the vectors' width.
+template <typename... Ps>
+bool aligned(size_t bytes, Ps... p) {
+    return ((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...);
+}
+size_t size_of(int dtype) { return dtype == DOT_I64 ? 8 : dtype == DOT_F32 || dtype == DOT_I32 ? 4 : 2; }
+
+int check_norm_addresses(const GroupNormArgs& a, const void* ws) {
+    if (!aligned(8, a.stats, ws)) return fail(DOT_ERR_INVALID, "stats and workspace must be 8-byte aligned");
+    if (!aligned(size_of(a.dtype), a.x, a.dy, a.y, a.dx) || !aligned(4, a.lengths) ||
+        !aligned(size_of(a.param_dtype), a.weight, a.bias, a.dweight, a.dbias))
+        return fail(DOT_ERR_INVALID, "tensor address not aligned to its elements");
+    return DOT_OK;
+}
+
 // Sizes, group count and types common to the forward and the backward.
 int check_norm(int dtype, int param_dtype, int64_t N, int64_t S, int64_t C, int64_t G, int activation) {
     if (N < 0 || S < 0 || C < 0) return fail(DOT_ERR_INVALID, "negative dimension");
@@ -69,6 +85,8 @@ int dot_group_norm_fwd(const void* x, int dtype, int64_t x_batch_stride, int64_t
     a.param_dtype = param_dtype;
     a.act = activation;
     a.eps = eps;
+    const int at = check_norm_addresses(a, workspace);
+    if (at) return at;
     return gn_run(a, workspace, false, static_cast<cudaStream_t>(stream));
 }
 
@@ -113,6 +131,8 @@ int dot_group_norm_bwd(const void* x, int dtype, int64_t x_batch_stride, int64_t
     a.dtype = dtype;
     a.param_dtype = param_dtype;
     a.act = activation;
+    const int at = check_norm_addresses(a, workspace);
+    if (at) return at;
     return gn_run(a, workspace, true, st);
 }
 
@@ -134,6 +154,9 @@ int dot_rotary(const void* q, const int64_t* q_strides, int64_t Hq, const void* 
     if ((Hq > 0 && (!q || !q_out || !q_strides)) || (Hk > 0 && (!k || !k_out || !k_strides)) || !positions ||
         !pos_strides || (P > 0 && !freqs))
         return fail(DOT_ERR_INVALID, "null tensor pointer");
+    if ((Hq > 0 && !aligned(size_of(dtype), q, q_out)) || (Hk > 0 && !aligned(size_of(dtype), k, k_out)) ||
+        !aligned(size_of(pos_dtype), positions) || !aligned(4, freqs))
+        return fail(DOT_ERR_INVALID, "tensor address not aligned to its elements");
     RotaryArgs a{};
     a.q = q;
     a.k = k;

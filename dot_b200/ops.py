@@ -329,7 +329,8 @@ def group_norm_backward_raw(x: torch.Tensor, dy: torch.Tensor, num_groups: int, 
     _check_norm_raw(x, num_groups, weight, bias, lengths)
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must have x's shape, dtype and device")
-    if stats.dtype != torch.float32 or stats.numel() < 2 * x.size(0) * num_groups or not stats.is_contiguous():
+    if stats.dtype != torch.float32 or stats.numel() < 2 * x.size(0) * num_groups or not stats.is_contiguous() or \
+            stats.device != x.device:
         raise ValueError("stats must be what group_norm_forward_raw returned")
     x, N, S, C, xb, xp = _rows(x)
     dy, _, _, _, gb, gp = _rows(dy)

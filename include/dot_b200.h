@@ -365,6 +365,9 @@ DOT_API int dot_bidir_bwd(const void* sim, int sim_dtype, const int32_t* lengths
 
 /* ------------------------------------------------------------------------ */
 /* Feature operators (no counterpart in the reference)                       */
+/*                                                                           */
+/* Tensors may start at any element; stats and workspace are 8-byte aligned  */
+/* (DOT_ERR_INVALID otherwise).                                              */
 /* ------------------------------------------------------------------------ */
 
 /* Bytes of workspace dot_group_norm_fwd / _bwd need for this problem. */
