@@ -1335,7 +1335,9 @@ size_t carve(void* ws, GnPlan& pl, bool backward) {
     return cv.size();
 }
 
-// Workspace of either path and any element type.
+// Workspace of either path and any element type.  The resident path needs none
+// forward; backward its chunks are at most a cluster's, a sample's positions, and
+// the SMs there are for each sample.
 size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward) {
     GnPlan pl{};
     pl.a.N = N;
@@ -1344,7 +1346,9 @@ size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward
     pl.a.G = G;
     sweep_plan(pl);
     const size_t sweeps = carve(nullptr, pl, backward);
-    pl.chunks = kMaxCluster;   // resident: needs none forward
+    int64_t chunks = kSMs / N < S ? kSMs / N : S;
+    if (chunks > kMaxCluster) chunks = kMaxCluster;
+    pl.chunks = int(chunks);
     const size_t resident = backward ? carve(nullptr, pl, true) : 0;
     return sweeps > resident ? sweeps : resident;
 }
