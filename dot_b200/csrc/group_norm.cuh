@@ -1356,27 +1356,33 @@ size_t workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G, bool backward
 // How a launch stands to the one before it, or to its own blocks.
 enum LaunchKind { kPlain, kDependent, kCooperative };
 
-// Whether the device takes a cooperative launch of one block for each of kSMs SMs.
-bool cooperative_device() {
-    static int known[64] = {};   // 0: not asked yet, 1: yes, -1: no
+// What has been asked of a device is kept, for each of them; calls come from any thread.
+constexpr int kMaxDevices = 64;
+
+// The current device if it takes a cooperative launch of one block for each of kSMs SMs, else -1.
+int cooperative_device() {
+    static std::atomic<int> known[kMaxDevices];   // 0: not asked yet, 1: yes, -1: no
     int dev = 0, sms = 0, coop = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    if (known[dev] == 0) {
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
+    int answer = known[dev].load(std::memory_order_relaxed);
+    if (answer == 0) {
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         cudaDeviceGetAttribute(&coop, cudaDevAttrCooperativeLaunch, dev);
-        known[dev] = sms >= kSMs && coop ? 1 : -1;
+        answer = sms >= kSMs && coop ? 1 : -1;
+        known[dev].store(answer, std::memory_order_relaxed);
     }
-    return known[dev] > 0;
+    return answer > 0 ? dev : -1;
 }
 
 // Whether a launch's clusters can all run at the same time, so that its blocks
-// may wait for one another (asked once for each kernel and cluster size).
+// may wait for one another (asked once for each device, kernel and cluster size).
 template <void (*kernel)(GnPlan)>
 bool all_at_once(int64_t blocks, int threads, size_t smem, int cluster) {
-    if (!cooperative_device()) return false;
+    const int dev = cooperative_device();
+    if (dev < 0) return false;
     if (cluster == 1) return blocks <= kSMs;
-    static std::atomic<int> known[kMaxCluster + 1];   // this kernel's clusters of each size; 0: not asked yet
-    int most = known[cluster].load(std::memory_order_relaxed);
+    static std::atomic<int> known[kMaxDevices][kMaxCluster + 1];   // this kernel's clusters; 0: not asked yet
+    int most = known[dev][cluster].load(std::memory_order_relaxed);
     if (most == 0) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(unsigned(cluster * kSMs));
@@ -1392,7 +1398,7 @@ bool all_at_once(int64_t blocks, int threads, size_t smem, int cluster) {
             cudaGetLastError();
             most = -1;
         }
-        known[cluster].store(most, std::memory_order_relaxed);
+        known[dev][cluster].store(most, std::memory_order_relaxed);
     }
     return threads <= kGnThreads && smem <= 48 * 1024 && blocks / cluster <= most;
 }
@@ -1531,7 +1537,7 @@ bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
     sweep_plan(pl);
     const int64_t blocks = a.N * pl.chunks;
     const bool waits = backward || pl.chunks > 1;
-    if (waits && (blocks > kSMs || !cooperative_device())) return false;
+    if (waits && (blocks > kSMs || cooperative_device() < 0)) return false;
     carve(ws, pl, backward);
     const size_t part = size_t(kGnThreads) * (backward || !ONEG ? VEC : 1) * sizeof(float2);
     const size_t groups = size_t(a.G + 1) * (backward ? sizeof(float4) + sizeof(float2) : sizeof(float2) + sizeof(float));
