@@ -1403,6 +1403,11 @@ bool all_at_once(int64_t blocks, int threads, size_t smem, int cluster) {
     return threads <= kGnThreads && smem <= 48 * 1024 && blocks / cluster <= most;
 }
 
+// What launch() answers where the blocks of a cooperative launch cannot all run at
+// once although the device could hold them: the stream's context has fewer SMs (a
+// partition of the device).  Nothing was launched.
+constexpr int kTooLarge = 1;
+
 // smem: dynamic, beside `merges` static bytes.  The opt-in is the kernel's and not the
 // launch's: all calls, from any thread, set it to the same most.
 template <typename K>
@@ -1438,7 +1443,10 @@ int launch(K kernel, const GnPlan& pl, int64_t blocks, int threads, size_t smem,
     }
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(n);
-    cudaLaunchKernelEx(&cfg, kernel, pl);
+    if (cudaLaunchKernelEx(&cfg, kernel, pl) == cudaErrorCooperativeLaunchTooLarge) {
+        cudaGetLastError();
+        return kTooLarge;
+    }
     return check_launch("group norm");
 }
 
@@ -1496,6 +1504,10 @@ int resident_run(GnPlan& pl, void* ws, int threads, bool backward, cudaStream_t 
         pl.share = (pl.a.dweight || pl.a.dbias) && all_at_once<kernel>(blocks, threads, smem, pl.chunks);
         ProfScope ps(DOT_K_NORM_BWD, st);
         rc = launch(kernel, pl, blocks, threads, smem, 0, pl.chunks, pl.share ? kCooperative : kPlain, st);
+        if (rc == kTooLarge) {
+            pl.share = 0;
+            rc = launch(kernel, pl, blocks, threads, smem, 0, pl.chunks, kPlain, st);
+        }
     }
     if (rc || pl.share) return rc;
     return launch_params(pl, st);
@@ -1528,7 +1540,8 @@ int sweep_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st) {
 
 // Both sweeps in one launch, where the rows lie one after another in memory, a
 // row's vectors are at most one per thread, the groups leave the ring its shared
-// memory, and every block that waits for others has an SM of its own.
+// memory, and every block that waits for others has an SM of its own; false where
+// that does not hold.
 template <typename T, int VEC, int ACT, bool ONEG>
 bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
     const GroupNormArgs& a = pl.a;
@@ -1546,7 +1559,7 @@ bool fused_run(GnPlan& pl, void* ws, bool backward, cudaStream_t st, int& rc) {
                            Ring<2>::bytes() + groups + part, kSmemMerges, 1, kCooperative, st)
                   : launch(gn_fused_fwd_kernel<T, VEC, ACT, ONEG>, pl, blocks, kGnThreads,
                            Ring<1>::bytes() + groups + part, kSmemMerges, 1, waits ? kCooperative : kPlain, st);
-    return true;
+    return rc != kTooLarge;
 }
 
 template <typename T, int VEC, int ACT, bool ONEG>
