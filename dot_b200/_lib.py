@@ -11,6 +11,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 import torch
 
@@ -104,16 +105,34 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-def load_torch_binding():
-    """The torch binding of the feature operators (``_lib/_torch_features.so``)."""
+_binding = None
+_binding_lock = threading.Lock()
+
+
+def torch_binding():
+    """The torch binding of the feature operators (``_lib/_torch_features.so``), loaded at their first
+    call: what needs the C-ABI library alone imports and runs without it."""
+    global _binding
+    if _binding is None:
+        with _binding_lock:
+            if _binding is None:
+                _binding = _load_torch_binding()
+    return _binding
+
+
+def _load_torch_binding():
     path = os.path.join(_HERE, "_lib", "_torch_features.so")
     if not os.path.exists(path):
         raise ImportError(f"dot_b200: torch binding not found at {path}; build it with `python dot_b200/build.py`")
     load()
-    loader = importlib.machinery.ExtensionFileLoader("_torch_features", path)
-    spec = importlib.util.spec_from_file_location("_torch_features", path, loader=loader)
-    module = importlib.util.module_from_spec(spec)
-    loader.exec_module(module)
+    try:
+        loader = importlib.machinery.ExtensionFileLoader("_torch_features", path)
+        spec = importlib.util.spec_from_file_location("_torch_features", path, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+    except ImportError as e:
+        raise ImportError(f"dot_b200: torch binding {path} does not load with torch {torch.__version__} ({e}); "
+                          "build it again with `python dot_b200/build.py`") from e
     return module
 
 

@@ -9,7 +9,7 @@ linked statically so the library carries no dependency beyond the driver
 ``csrc/torch_features.cpp``, the torch binding of the feature operators, is
 compiled with the host compiler against the installed torch and linked to that
 library (``_lib/_torch_features.so``).  Each is skipped when it is newer than
-its sources.
+its sources, the binding if it was also built for the torch and Python that run.
 """
 
 from __future__ import annotations
@@ -26,6 +26,7 @@ ROOT = os.path.dirname(HERE)
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIB_DIR, "libdot_b200.so")
 BINDING = os.path.join(LIB_DIR, "_torch_features.so")
+BINDING_STAMP = os.path.join(LIB_DIR, "_torch_features.built_for")   # the torch and Python it was compiled against
 BINDING_SRC = os.path.join(HERE, "csrc", "torch_features.cpp")
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
@@ -50,14 +51,25 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _binding_stale(built_for: str) -> bool:
+    if not os.path.exists(BINDING) or not os.path.exists(BINDING_STAMP):
+        return True
+    with open(BINDING_STAMP) as f:
+        if f.read() != built_for:
+            return True
+    deps = [BINDING_SRC, os.path.join(ROOT, "include", "dot_b200.h")]
+    return any(os.path.getmtime(d) > os.path.getmtime(BINDING) for d in deps)
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> str:
     """The torch binding: host code only, linked to libdot_b200.so beside it."""
-    deps = [BINDING_SRC, os.path.join(ROOT, "include", "dot_b200.h")]
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
-        return BINDING
     import sysconfig
 
     import torch
+
+    built_for = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+    if not force and not _binding_stale(built_for):
+        return BINDING
     from torch.utils import cpp_extension
 
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
@@ -75,6 +87,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
+    with open(BINDING_STAMP, "w") as f:
+        f.write(built_for)
     return BINDING
 
 

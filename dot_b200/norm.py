@@ -29,9 +29,6 @@ import torch.nn as nn
 
 from . import _lib
 
-_binding = _lib.load_torch_binding()
-
-
 _ACTIVATION_CODES = {name: code for code, name in enumerate(_lib.ACTIVATIONS)}
 
 
@@ -54,7 +51,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     Gradients for x, weight and bias (once differentiable, in reverse mode);
     forward-mode tangents and ``torch.jit.trace`` raise NotImplementedError.
     """
-    return _binding.group_norm_act(x, num_groups, weight, bias, eps, _activation_code(activation), lengths)
+    return _lib.torch_binding().group_norm_act(x, num_groups, weight, bias, eps, _activation_code(activation), lengths)
 
 
 class GroupNormAct(nn.Module):

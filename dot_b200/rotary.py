@@ -24,7 +24,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn as nn
 
-from .norm import _binding
+from . import _lib
 
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Optional[torch.Tensor] = None,
@@ -39,7 +39,7 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, k: Opt
     k is given.  Differentiable in q and k, not in positions or freqs;
     forward-mode tangents and ``torch.jit.trace`` raise NotImplementedError.
     """
-    q, turned_k = _binding.rotary(q, positions, freqs, k, interleaved)
+    q, turned_k = _lib.torch_binding().rotary(q, positions, freqs, k, interleaved)
     return q if k is None else (q, turned_k)
 
 
