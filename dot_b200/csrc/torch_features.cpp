@@ -49,8 +49,18 @@ void refuse_modes(const char* what, const Ts&... inputs) {
     TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "dot_b200: ", what, " has no forward-mode derivative");
 }
 
-const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// The address of a tensor that may be left out.  One that is there but has no memory (torch's
+// tensors of zeros without storage, fake ones) must not pass for one that is not.
+void* out(const Tensor& t) {
+    if (!t.defined()) return nullptr;
+    void* p = t.data_ptr();
+    TORCH_CHECK_VALUE(p != nullptr || t.numel() == 0, "dot_b200: a tensor without memory");
+    return p;
+}
+const void* ptr(const Tensor& t) { return out(t); }
+
+// The values as they are in memory: a view that torch negates when it is read is copied.
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
 optional<Tensor> present(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
@@ -65,7 +75,8 @@ void* current_stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t
 struct Rows {
     Tensor t;
     int64_t N, S, C, batch = 0, pos = 0;
-    explicit Rows(const Tensor& x) : t(x), N(x.size(0)), S(1), C(x.size(-1)) {
+    explicit Rows(const Tensor& x_in) : t(plain(x_in)), N(t.size(0)), S(1), C(t.size(-1)) {
+        const Tensor x = t;
         const int64_t dims = x.dim();
         for (int64_t d = 1; d < dims - 1; ++d) S *= x.size(d);
         if (x.numel() == 0) return;
@@ -170,7 +181,7 @@ Tensor norm_param(const optional<Tensor>& p, const Tensor& x, const char* name) 
     const int64_t C = x.size(-1);
     TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == C, name, " must have shape [", C, "]");
     TORCH_CHECK_VALUE(p->device() == x.device(), name, " must be on ", x.device());
-    return p->contiguous();
+    return plain(p->contiguous());
 }
 
 Tensor group_norm_act(const Tensor& x, int64_t groups, const optional<Tensor>& weight, const optional<Tensor>& bias,
@@ -215,16 +226,18 @@ int position_dtype(at::ScalarType t) {
 
 // q [B,L,Hq,D] and/or k [B,L,Hk,D] (either may be undefined) turned by the
 // angles of positions [B or 1, L, A] and freqs [P,A].
-std::pair<Tensor, Tensor> turn(const Tensor& q_in, const Tensor& k_in, const Tensor& positions, const Tensor& freqs,
-                               bool interleaved, bool inverse) {
+std::pair<Tensor, Tensor> turn(const Tensor& q_in, const Tensor& k_in, const Tensor& positions_in,
+                               const Tensor& freqs_in, bool interleaved, bool inverse) {
     const Tensor& ref = q_in.defined() ? q_in : k_in;
     const c10::cuda::CUDAGuard guard(ref.device());
+    const Tensor positions = plain(positions_in), freqs = plain(freqs_in);
     const int64_t D = ref.size(3);
     Tensor q, k, qo, ko;
     int64_t qs[3] = {}, ks[3] = {}, ps[3];
     auto take = [&](const Tensor& in, Tensor& t, Tensor& o, int64_t* s) {
         if (!in.defined()) return;
-        t = D == 1 || in.stride(3) == 1 ? in : in.contiguous();   // elements of a head are consecutive
+        t = plain(in);
+        if (D > 1 && t.stride(3) != 1) t = t.contiguous();   // elements of a head are consecutive
         o = dense_like(in);
         for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
     };
@@ -233,8 +246,8 @@ std::pair<Tensor, Tensor> turn(const Tensor& q_in, const Tensor& k_in, const Ten
     for (int i = 0; i < 3; ++i) ps[i] = positions.stride(i);
     if (positions.size(0) != ref.size(0)) ps[0] = 0;
     check(dot_rotary(ptr(q), qs, q.defined() ? q.size(2) : 0, ptr(k), ks, k.defined() ? k.size(2) : 0,
-                     feature_dtype(ref.scalar_type()), positions.data_ptr(), position_dtype(positions.scalar_type()),
-                     ps, static_cast<const float*>(freqs.data_ptr()), ref.size(0), ref.size(1), D, freqs.size(0),
+                     feature_dtype(ref.scalar_type()), ptr(positions), position_dtype(positions.scalar_type()),
+                     ps, static_cast<const float*>(ptr(freqs)), ref.size(0), ref.size(1), D, freqs.size(0),
                      int(freqs.size(1)), interleaved, inverse, out(qo), out(ko), current_stream(ref)),
           "dot_rotary");
     return {qo, ko};

@@ -1,6 +1,7 @@
-"""Ways of calling the feature operators that their torch binding cannot serve:
-a tangent of forward-mode differentiation and a trace are refused, not passed
-by.  The refusals come before the device is looked at, so most need no GPU."""
+"""Tensors and ways of calling that a binding working on memory could pass by: a
+tangent of forward-mode differentiation and a trace are refused (before the device
+is looked at, so most of it needs no GPU), a view that torch negates when it is read
+counts as what it stands for, one without memory is refused."""
 
 import pytest
 import torch
@@ -60,3 +61,41 @@ def test_tangents_of_upstream_gradients_are_refused():
                     torch.autograd.grad(y, leaf, up, retain_graph=True, create_graph=create)
         (g,) = torch.autograd.grad(y, leaf, torch.ones_like(y))   # and without one the gradient is there
         assert g.shape == leaf.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(7))
+def test_negated_views(i):
+    t, call = calls("cuda")[i]
+    view = torch._neg_view(t)
+    assert view.is_neg() and torch.equal(call(view)[0], call(-t)[0])
+
+
+@pytest.mark.gpu
+def test_negated_views_of_complex_numbers():
+    """Imaginary parts of conjugates, as positions in place and as the single channel of an input."""
+    z = torch.randn(3, 2, 2, device="cuda")
+    z = torch.view_as_complex(z).conj()
+    q = torch.rand(1, 3, 2, 8, device="cuda")
+    assert z.imag.is_neg()
+    assert torch.equal(dot.rotary(q, z.imag, FREQS.cuda()), dot.rotary(q, z.imag.clone(), FREQS.cuda()))
+    x = z.imag[..., None]
+    assert torch.equal(dot.group_norm_act(x, 1), dot.group_norm_act(x.clone(), 1))
+
+
+@pytest.mark.gpu
+def test_negated_upstream_gradients():
+    x = torch.rand(2, 3, 8, device="cuda", requires_grad=True)
+    q = torch.rand(1, 3, 2, 8, device="cuda", requires_grad=True)
+    for leaf, y in ((x, dot.group_norm_act(x, 2)), (q, dot.rotary(q, POS.cuda(), FREQS.cuda()))):
+        dy = torch.rand_like(y)
+        got, want = (torch.autograd.grad(y, leaf, g, retain_graph=True)[0] for g in (torch._neg_view(dy), -dy))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(7))
+def test_tensors_without_memory_are_refused(i):
+    t, call = calls("cuda")[i]
+    with pytest.raises(ValueError):
+        call(torch._efficientzerotensor(tuple(t.shape), device="cuda"))
