@@ -345,9 +345,10 @@ struct Place {
 // stage holds U rows for each row position of the block, of x and for NT = 2 of
 // dy; the last of the 16 warps to leave a stage refills it.  Waits are bounded.
 // A thread whose wait expired goes on without waiting and writes NaN, into every
-// channel of its partial sums on the way in and of its rows on the way out; the
-// block starts no further copy, since the barrier of the lost one is still in its
-// phase, and before it ends waits (again with a limit) for those in flight.
+// channel of its partial sums on the way in and of its rows on the way out; its
+// warp leaves no stage any more, so that the block starts no further copy (the
+// barrier of the lost one is still in its phase), and before it ends it waits
+// (again with a limit) for those in flight.
 constexpr int kRingStages = 5;
 constexpr int kRingStageBytes = 32 * 1024;
 
@@ -364,14 +365,12 @@ struct Ring {
     uint64_t* full;                     // [kRingStages]
     int* left;                          // [kRingStages] warps that have left the stage
     int* copies;                        // [kRingStages] copies started into the slot
-    volatile int* lost;                 // a wait expired: no copy is started any more
     const unsigned char* src[NT];       // row 0 of the block's range
     int row_bytes, rows, stage_rows, n; // rows in all, per stage; stages
     bool dead = false;
 
     static constexpr size_t bytes() {   // what follows is 16-byte aligned
-        const size_t stage = kRingStageBytes + sizeof(uint64_t) + 2 * sizeof(int);
-        return (size_t(kRingStages) * stage + sizeof(int) + 15) / 16 * 16;
+        return (size_t(kRingStages) * (kRingStageBytes + sizeof(uint64_t) + 2 * sizeof(int)) + 15) / 16 * 16;
     }
     // By all threads, before a block barrier.
     __device__ __forceinline__ void init(unsigned char* smem, int rows_, int stage_rows_, int row_bytes_) {
@@ -379,7 +378,6 @@ struct Ring {
         full = reinterpret_cast<uint64_t*>(smem + kRingStages * kRingStageBytes);
         left = reinterpret_cast<int*>(full + kRingStages);
         copies = left + kRingStages;
-        lost = copies + kRingStages;
         rows = rows_;
         stage_rows = stage_rows_;
         row_bytes = row_bytes_;
@@ -390,7 +388,6 @@ struct Ring {
                 mbar_init(full + k, 1);
                 left[k] = copies[k] = 0;
             }
-            *lost = 0;
             mbar_fence_init();
         }
     }
@@ -416,21 +413,18 @@ struct Ring {
     // A warp leaves stage i; the last one brings stage `next` into its place, its c-th copy.
     __device__ __forceinline__ void leave(int i, int next, int c) {
         const int slot = i % kRingStages;
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) {
+        if (!__any_sync(0xffffffffu, dead) && (threadIdx.x & 31) == 0) {
             __threadfence_block();
             if (atomicAdd(left + slot, 1) == kGnWarps - 1) {
                 left[slot] = 0;
                 __threadfence_block();
                 fence_proxy_async_smem();
-                if (!*lost) issue(next, c);   // set before the warp that set it left
+                issue(next, c);
             }
         }
     }
     __device__ __forceinline__ void wait(int i) {
-        if (dead || mbar_wait_sleep(full + i % kRingStages, uint32_t(i / kRingStages) & 1u, nullptr)) return;
-        dead = true;
-        *lost = 1;
+        if (!dead) dead = !mbar_wait_sleep(full + i % kRingStages, uint32_t(i / kRingStages) & 1u, nullptr);
     }
     // use(stage's bytes, its first row, its rows), first stage to last.  The
     // c-th copy into a slot completes its barrier's phase c: stage i is copy
@@ -455,10 +449,12 @@ struct Ring {
                 leave(i, i - kRingStages, (n - 1 - i % kRingStages) / kRingStages * 2 - i / kRingStages + 1);
         }
     }
-    // At the end, by all threads: copies still in flight must not outlive the block.
+    // At the end: copies still in flight must not outlive the block.  Whichever thread
+    // started one has either seen it arrive or waits for it here.
     __device__ __forceinline__ void drain() {
-        if (__syncthreads_or(dead) && threadIdx.x < kRingStages && copies[threadIdx.x] > 0)
-            mbar_wait_sleep(full + threadIdx.x, uint32_t(copies[threadIdx.x] - 1) & 1u, nullptr);
+        if (dead)
+            for (int k = 0; k < min(n, kRingStages); ++k)
+                if (copies[k] > 0) mbar_wait_sleep(full + k, uint32_t(copies[k] - 1) & 1u, nullptr);
     }
 };
 
