@@ -18,8 +18,8 @@
 // has a fixed order, so results are bitwise reproducible.
 //
 // Measured (device time, 6.55 TB/s copy rate): 8 x 4800 x 256 bfloat16 with silu
-// 16.7 us forward; 16 x 76800 x 64 with relu 81.7 us; 2 x 76800 x 256 with silu
-// 45.5 us forward and 72.1 backward; 16 x 1024 x 256 padded sets 7.8 and 14.1.
+// 16.6 us forward; 16 x 76800 x 64 with relu 82.2 us; 2 x 76800 x 256 with silu
+// 45.9 us forward and 72.6 backward; 16 x 1024 x 256 padded sets 7.9 and 14.0.
 //
 // Moments are kept as (mean, sum M of squared deviations) of x - pivot, the
 // pivot one of the group's values: a mean far from zero then costs its own
@@ -896,8 +896,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_dx_kernel(GnPlan pl) {
 // grid barrier between them where a sample's chunks lie in several blocks (a
 // cooperative launch, one block per SM), so the second one finds the last 160 KB
 // of every block's rows on chip and no launch lies between them.  Against two
-// launches with plain loads: 8 x 4800 x 256 18.9 -> 16.7 us, clip backward 90 ->
-// 72.  HBM bounds the way forwards (6.3 TB/s with the write-backs of earlier
+// launches with plain loads: 8 x 4800 x 256 18.9 -> 16.6 us, clip backward 90 ->
+// 73.  HBM bounds the way forwards (6.3 TB/s with the write-backs of earlier
 // results).  The way back of 79 MB takes 20 us: 16 without silu, 16 without the
 // stores, 16 us of HBM and L2 traffic in either case; where x exceeds L2 HBM
 // bounds it too (157 MB read and written: 6.2 TB/s).
@@ -1090,8 +1090,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) gn_fused_bwd_kernel(GnPlan pl) 
 // gradients, which cross clusters, follow a grid barrier at the end where all
 // clusters run at once (a launch of their own costs a training call 7 us of 73
 // on the host and saves 1 us of 14 on the device), else they are a second
-// launch.  Bound by latency: 3.4 us for one 64 x 64 sample, 7.8 us forward and
-// 14.1 us backward for 8.4 MB.
+// launch.  Bound by latency: 3.5 us for one 64 x 64 sample, 7.9 us forward and
+// 14.0 us backward for 8.4 MB.
 
 // Where a block stands: chunk (its rank in the cluster), slab, sample.
 struct ResPlace {
